@@ -1,0 +1,266 @@
+"""ops.heads and ops.distill on the CPU: the references against loops over their definitions, their
+gradients against differences, and what the entry points refuse."""
+import math
+
+import pytest
+import torch
+
+from metaopt_amd.ops import distill, heads, lm
+
+
+def _rand(*shape, dtype=torch.float64):
+    return torch.randn(*shape, dtype=dtype)
+
+
+# ------------------------------------------------------------------------------- definitions
+@pytest.mark.parametrize("il", [False, True])
+def test_qk_norm_rope_is_the_formula(il):
+    torch.manual_seed(0)
+    P, n, T, H, KV, D = 2, 4, 3, 4, 2, 8
+    qkv, wq, wk = _rand(n * T, (H + 2 * KV) * D), _rand(P, D), _rand(P, D)
+    cos, sin = heads.rope_tables(8, D)
+    q, k, v = heads.qk_norm_rope(qkv, wq, wk, cos, sin, T, H, KV, eps=1e-3, il=il)
+    for b in range(n):
+        for t in range(T):
+            for h in range(H + 2 * KV):
+                x = qkv[b * T + t, h * D:(h + 1) * D]
+                if h >= H + KV:
+                    assert torch.equal(v[b, h - H - KV, t], x)
+                    continue
+                w = (wq if h < H else wk)[b // (n // P)]
+                y = x / math.sqrt(float((x * x).mean()) + 1e-3) * w
+                z = torch.empty(D, dtype=torch.float64)
+                for j in range(D // 2):
+                    i0, i1 = (2 * j, 2 * j + 1) if il else (j, j + D // 2)
+                    c, s = float(cos[t, j]), float(sin[t, j])
+                    z[i0], z[i1] = y[i0] * c - y[i1] * s, y[i1] * c + y[i0] * s
+                got = q[b, h, t] if h < H else k[b, h - H, t]
+                torch.testing.assert_close(got, z, rtol=1e-12, atol=1e-12)
+
+
+def test_qk_norm_rope_gradients_match_differences():
+    torch.manual_seed(1)
+    P, n, T, H, KV, D = 2, 2, 3, 2, 1, 4
+    cos, sin = heads.rope_tables(T, D)
+    args = [t.requires_grad_(True) for t in (_rand(n * T, (H + 2 * KV) * D), _rand(P, D), _rand(P, D))]
+    for il in (False, True):
+        assert torch.autograd.gradcheck(
+            lambda x, a, b: heads.qk_norm_rope(x, a, b, cos, sin, T, H, KV, il=il), args)
+
+
+@pytest.mark.parametrize("T", [1, 2])
+def test_cached_heads_are_the_whole_sequence_s(T):
+    """Tokens added T at a time leave in the cache what one call over the sequence gives."""
+    torch.manual_seed(2)
+    P, n, L, H, KV, D = 2, 4, 6, 4, 2, 8
+    qkv, wq, wk = _rand(n * L, (H + 2 * KV) * D), _rand(P, D), _rand(P, D)
+    cos, sin = heads.rope_tables(L, D)
+    want = heads.qk_norm_rope(qkv, wq, wk, cos, sin, L, H, KV)
+    kc, vc = torch.full((n, KV, L + 2, D), 9.0, dtype=torch.float64), \
+        torch.full((n, KV, L + 2, D), 9.0, dtype=torch.float64)
+    for t in range(0, L, T):
+        rows = qkv.view(n, L, -1)[:, t:t + T].reshape(n * T, -1)
+        start = torch.full((n,), t, dtype=torch.int32)
+        q = heads.qk_norm_rope_cached(rows, wq, wk, cos, sin, T, H, kc, vc, start)
+        torch.testing.assert_close(q, want[0][:, :, t:t + T])
+    torch.testing.assert_close(kc[:, :, :L], want[1])
+    torch.testing.assert_close(vc[:, :, :L], want[2])
+    assert (kc[:, :, L:] == 9).all() and (vc[:, :, L:] == 9).all()
+
+
+def test_cached_heads_leave_out_positions_that_are_not_there():
+    torch.manual_seed(3)
+    n, T, H, D, cap = 4, 2, 2, 8, 5
+    rows, w = _rand(n * T, 3 * H * D), _rand(1, D)
+    cos, sin = heads.rope_tables(4, D)
+    kc, vc = torch.zeros(n, H, cap, D, dtype=torch.float64), torch.zeros(n, H, cap, D, dtype=torch.float64)
+    start = torch.tensor([-1, 3, 4, 0], dtype=torch.int32)
+    q = heads.qk_norm_rope_cached(rows, w, w, cos, sin, T, H, kc, vc, start)
+    there = {(0, 1): 0, (1, 0): 3, (3, 0): 0, (3, 1): 1}      # (sequence, token): position
+    for b in range(n):
+        for t in range(T):
+            assert (q[b, :, t].abs().sum() > 0) == ((b, t) in there)
+    written = [(b, p) for b in range(n) for p in range(cap) if kc[b, :, p].abs().sum() > 0]
+    assert written == sorted((b, p) for (b, _), p in there.items())
+
+
+def _naive_attention(q, k, v, window, sinks, scale, start, lengths):
+    B, H, Tq, D = q.shape
+    KV, Tk = k.shape[1:3]
+    o = torch.zeros(B, Tq, H, D, dtype=torch.float64)
+    for b in range(B):
+        for h in range(H):
+            for t in range(Tq):
+                i = start[b] + t
+                js = [j for j in range(min(Tk, lengths[b])) if 0 <= i < min(Tk, lengths[b]) and j <= i
+                      and (window is None or i - j < window or j < sinks)]
+                if js:
+                    kk, vv = k[b, h // (H // KV), js], v[b, h // (H // KV), js]
+                    p = (kk @ q[b, h, t] * scale).softmax(0)
+                    o[b, t, h] = p @ vv
+    return o.view(B * Tq, H * D)
+
+
+@pytest.mark.parametrize("Tq,Tk,window,sinks,start,lengths", [
+    (5, 5, None, 0, None, None), (6, 6, 2, 0, None, None), (7, 7, 2, 1, None, [0, 1, 7]),
+    (7, 7, 1, 3, None, [4, 9, 2]), (2, 9, 3, 2, None, None), (1, 9, 4, 1, [0, 5, 8], None),
+    (3, 6, 2, 2, [-1, 5, 9], None), (3, 6, 2, 2, -2, None), (4, 6, 3, 1, [0, 1, 2], [2, 3, 6])])
+def test_window_attention_is_the_formula(Tq, Tk, window, sinks, start, lengths):
+    torch.manual_seed(4)
+    B, H, KV, D = 3, 4, 2, 8
+    q, k, v = _rand(B, H, Tq, D), _rand(B, KV, Tk, D), _rand(B, KV, Tk, D)
+    first = [Tk - Tq] * B if start is None else start if isinstance(start, list) else [start] * B
+    last = [f + Tq for f in first] if lengths is None else lengths
+    tensor = lambda x: torch.tensor(x, dtype=torch.int32) if isinstance(x, list) else x  # noqa: E731
+    o = heads.window_attention(q, k, v, window, sinks, start=tensor(start), lengths=tensor(lengths))
+    want = _naive_attention(q, k, v, window, sinks, 1 / math.sqrt(D), first, last)
+    torch.testing.assert_close(o, want, rtol=1e-12, atol=1e-12)
+
+
+def test_window_attention_ignores_what_padding_holds():
+    torch.manual_seed(5)
+    B, H, T, D = 2, 2, 6, 8
+    q, k, v = (_rand(B, H, T, D) for _ in range(3))
+    lengths = torch.tensor([3, 0], dtype=torch.int32)
+    want = heads.window_attention(q, k, v, 2, 1, lengths=lengths)
+    leaves = []
+    for t in (q, k, v):
+        t = t.clone()
+        t[0, :, 3:], t[1] = float("nan"), float("inf")
+        leaves.append(t.requires_grad_(True))
+    got = heads.window_attention(*leaves, 2, 1, lengths=lengths)
+    assert torch.equal(got, want) and (got.view(B, T, -1)[0, 3:] == 0).all()
+    for g in torch.autograd.grad(got[:3].sum(), leaves):
+        assert torch.isfinite(g).all() and (g[0, :, 3:] == 0).all() and (g[1] == 0).all()
+
+
+def test_window_attention_gradients_match_differences():
+    torch.manual_seed(6)
+    q, k, v = _rand(2, 4, 5, 3), _rand(2, 2, 5, 3), _rand(2, 2, 5, 3)
+    lengths = torch.tensor([5, 3], dtype=torch.int32)
+    assert torch.autograd.gradcheck(
+        lambda a, b, c: heads.window_attention(a, b, c, 2, 1, lengths=lengths),
+        [t.requires_grad_(True) for t in (q, k, v)])
+
+
+def test_plain_causal_window_is_lm_attention():
+    torch.manual_seed(7)
+    q, k, v = (_rand(2, 3, 64, 64, dtype=torch.float32) for _ in range(3))
+    torch.testing.assert_close(heads.window_attention(q, k, v), lm.attention(q, k, v))
+
+
+def _naive_distill(x, y, t, index, tau, a):
+    V = len(x)
+    lp1, lpt = x.log_softmax(0), (x / tau).log_softmax(0)
+    loss = 0.0
+    if 0 <= y < V:
+        loss += (1 - a) * -float(lp1[y])
+    there = [k for k, i in enumerate(index) if 0 <= i < V]
+    if there:
+        lq = (t[there] / tau).log_softmax(0)
+        loss += a * tau * tau * sum(float(l.exp() * (l - lpt[index[k]])) for l, k in zip(lq, there))
+    return loss
+
+
+def test_distill_loss_is_the_formula():
+    torch.manual_seed(8)
+    P, rows, V, K = 2, 4, 11, 3
+    x, t = _rand(P * rows, V), _rand(P * rows, K)
+    index = torch.randint(0, V, (P * rows, K), dtype=torch.int32)
+    index[1] = -1
+    index[2, 1] = V
+    index[3] = index[3, 0]                                   # one place three times
+    y = torch.randint(0, V, (P * rows,), dtype=torch.int32)
+    y[1], y[5] = -100, V
+    tau, a = torch.tensor([1.0, 2.5]), torch.tensor([0.25, 1.0])
+    got = distill.distill_loss(x, y, t, index, rows, tau, a)
+    for p in range(P):
+        want = sum(_naive_distill(x[r], int(y[r]), t[r], index[r].tolist(), float(tau[p]), float(a[p]))
+                   for r in range(p * rows, (p + 1) * rows))
+        assert abs(float(got[p]) - want) < 1e-10
+
+
+def test_distill_loss_gradients_match_differences():
+    torch.manual_seed(9)
+    x, t = _rand(4, 7).requires_grad_(True), _rand(4, 3)
+    index = torch.tensor([[0, 1, 1], [-1, 2, 6], [-1, -1, -1], [5, 5, 5]], dtype=torch.int32)
+    y = torch.tensor([0, -1, 3, 6], dtype=torch.int32)
+    assert torch.autograd.gradcheck(
+        lambda z: distill.distill_loss(z, y, t, index, 2, 1.7, 0.4), [x])
+    grad, = torch.autograd.grad(distill.distill_loss(x, y, t, index, 2, 1.7, 0.4).sum(), x)
+    scaled, = torch.autograd.grad(
+        distill.distill_loss(x, y, t, index, 2, 1.7, 0.4, grad_scale=0.5).sum(), x)
+    torch.testing.assert_close(scaled, 0.5 * grad)
+
+
+def test_distill_without_teacher_is_cross_entropy():
+    torch.manual_seed(10)
+    x = _rand(6, 9, dtype=torch.float32)
+    y = torch.randint(0, 9, (6,), dtype=torch.int32)
+    none = torch.empty(6, 0), torch.empty(6, 0, dtype=torch.int32)
+    got = distill.distill_loss(x, y, *none, 3, alpha=0.0)
+    torch.testing.assert_close(got, lm.cross_entropy(x, y, 3))
+
+
+# ------------------------------------------------------------------------------- refusals
+def _qk_args(**kw):
+    d = dict(qkv=torch.zeros(4, 32), wq=torch.ones(1, 8), wk=torch.ones(1, 8),
+             cos=torch.zeros(2, 4), sin=torch.zeros(2, 4), T=2, H=2)
+    return dict(d, **kw)
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(qkv=torch.zeros(4, 33)), "columns"), (dict(qkv=torch.zeros(5, 48)), "whole sequences"),
+    (dict(qkv=torch.zeros(4, 48), T=0), "positive"), (dict(qkv=torch.zeros(4, 48), T=4), "tables"),
+    (dict(qkv=torch.zeros(4, 56), H=3, kv_heads=2), "multiple"),
+    (dict(qkv=torch.zeros(4, 48), cos=torch.zeros(2, 3)), "table"),
+    (dict(qkv=torch.zeros(4, 48), sin=torch.zeros(2, 4).double()), "table"),
+    (dict(qkv=torch.zeros(4, 48), wk=torch.ones(2, 8)), "trials"),
+    (dict(qkv=torch.zeros(4, 48).half()), "one type"), (dict(qkv=torch.zeros(2, 2, 48)), "rows")])
+def test_qk_norm_rope_refuses(bad, match):
+    with pytest.raises(ValueError, match=match):
+        heads.qk_norm_rope(**_qk_args(**bad))
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(start=torch.zeros(2)), "int32"), (dict(start=torch.zeros(3, dtype=torch.int32)), "int32"),
+    (dict(kcache=torch.zeros(2, 2, 4, 8), vcache=torch.zeros(2, 2, 5, 8)), "alike"),
+    (dict(kcache=torch.zeros(3, 2, 4, 8), vcache=torch.zeros(3, 2, 4, 8)), "sequences"),
+    (dict(kcache=torch.zeros(2, 2, 4, 8).half(), vcache=torch.zeros(2, 2, 4, 8).half()), "type")])
+def test_qk_norm_rope_cached_refuses(bad, match):
+    d = _qk_args(qkv=torch.zeros(4, 48), kcache=torch.zeros(2, 2, 4, 8), vcache=torch.zeros(2, 2, 4, 8),
+                 start=torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(ValueError, match=match):
+        heads.qk_norm_rope_cached(**dict(d, **bad))
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(q=torch.zeros(1, 3, 4, 8)), "multiple"), (dict(q=torch.zeros(2, 2, 4, 8)), "fit"),
+    (dict(q=torch.zeros(2, 4, 8)), "B, H"), (dict(q=torch.zeros(1, 2, 4, 8).half()), "one type"),
+    (dict(window=0), "window"), (dict(sinks=-1), "sinks"), (dict(scale=0.0), "positive"),
+    (dict(scale=float("inf")), "positive"), (dict(start=torch.zeros(1)), "int32"),
+    (dict(start=1 << 40), "position"), (dict(lengths=torch.zeros(2, dtype=torch.int32)), "int32"),
+    (dict(lengths=torch.zeros(1, dtype=torch.int64)), "int32")])
+def test_window_attention_refuses(bad, match):
+    d = dict(q=torch.zeros(1, 2, 4, 8), k=torch.zeros(1, 2, 4, 8), v=torch.zeros(1, 2, 4, 8))
+    with pytest.raises(ValueError, match=match):
+        heads.window_attention(**dict(d, **bad))
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(labels=torch.zeros(4)), "int32"), (dict(labels=torch.zeros(3, dtype=torch.int32)), "int32"),
+    (dict(top_index=torch.zeros(4, 2, dtype=torch.int64)), "int32"),
+    (dict(top_values=torch.zeros(4, 3)), "one shape"),
+    (dict(top_values=torch.zeros(4, 2, requires_grad=True)), "detach"),
+    (dict(top_values=torch.zeros(4, 1025), top_index=torch.zeros(4, 1025, dtype=torch.int32)), "1024"),
+    (dict(rows_per_trial=3), "whole trials"), (dict(temperature=0.0), "temperature"),
+    (dict(temperature=float("nan")), "temperature"), (dict(alpha=1.5), "alpha"),
+    (dict(alpha=torch.zeros(3)), "alpha"), (dict(alpha=torch.zeros(2).double()), "alpha"),
+    (dict(temperature=torch.ones(2, requires_grad=True)), "detach"), (dict(inplace=True), "unit_weights"),
+    (dict(logits=torch.zeros(4)), "vocabulary")])
+def test_distill_loss_refuses(bad, match):
+    d = dict(logits=torch.zeros(4, 5), labels=torch.zeros(4, dtype=torch.int32),
+             top_values=torch.zeros(4, 2), top_index=torch.zeros(4, 2, dtype=torch.int32),
+             rows_per_trial=2)
+    with pytest.raises(ValueError, match=match):
+        distill.distill_loss(**dict(d, **bad))
