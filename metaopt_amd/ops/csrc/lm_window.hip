@@ -98,27 +98,59 @@ __device__ __forceinline__ f32x16 zero16() {
   return f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 }
 
-// Staging of [BN][D] rows by 256 threads: rows outside [lo, hi) are zeros (never read)
+// ------------------------------------------------------------------------------------ staging
+// Tiles come from memory straight into LDS (global_load_lds: lane l of a wave fills bytes
+// 16 l ... of 1 KB), so the exchange of chunks is applied to the addresses that are read.  A ring of
+// NS tiles is filled NS - 1 ahead with one barrier a tile: the fills go through inline asm, where
+// the compiler does not see them and would wait for all of them before every transposing read, and
+// tile_wait waits for those of the next tile itself.  Rows outside [lo, hi) are read as the nearest
+// row inside (values of the sequence, finite as the others; the masks leave them out): what padding
+// holds is never read.
+typedef __attribute__((address_space(3))) void lds_void;
+
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)((lds_void*)p));
+}
+__device__ __forceinline__ void fill16(const void* src, const void* dst) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_at(dst)) : "memory", "m0");
+}
+__device__ __forceinline__ void fill4(const void* src, const void* dst) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds_at(dst)) : "memory", "m0");
+}
+
+// until at most N of this wave's loads are under way, then until every wave is there
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
 template <int D>
-struct Stage {
-  static constexpr int N = BN * D / 8 / 256;           // 16-byte chunks a thread
-  u32x4 r[N];
-  __device__ __forceinline__ void load(const uint16_t* g, int64_t ld, int row0, int lo, int hi, int tid) {
+constexpr int kFills = BN * D * 2 / 1024 / 4;          // 1 KB fills of a tile by each of 4 waves
+
+template <int D>
+__device__ __forceinline__ void fill_tile(const uint16_t* g, int64_t ld, int row0, int lo, int hi, uint16_t* img,
+                                          int wave, int lane) {
+  constexpr int CH = D / 8, PER = 64 / CH;             // chunks of a row, rows of a fill
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = tid + 256 * i, row = row0 + c / (D / 8);
-      r[i] = u32x4{0, 0, 0, 0};
-      if (row >= lo && row < hi) r[i] = *(const u32x4*)(g + (int64_t)row * ld + (c % (D / 8)) * 8);
-    }
+  for (int j = 0; j < kFills<D>; ++j) {
+    const int blk = wave * kFills<D> + j, r = blk * PER + lane / CH, c = (lane % CH) ^ swz<D>(r);
+    const int row = max(lo, min(hi - 1, row0 + r));
+    fill16(g + row * ld + c * 8, img + blk * 512);
   }
-  __device__ __forceinline__ void store(uint16_t* s, int tid) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = tid + 256 * i;
-      *(u32x4*)(s + at<D>(c / (D / 8), (c % (D / 8)) * 8)) = r[i];
-    }
-  }
-};
+}
+
+// waves a SIMD: the registers that a kernel may use (512 / waves)
+#ifndef MOPT_WINDOW_WAVES
+#define MOPT_WINDOW_WAVES 3, 2, 3, 2, 3, 2
+#endif
+constexpr int kWaves[6] = {MOPT_WINDOW_WAVES};
+template <int D> constexpr int kFwdWaves = kWaves[D == 128];
+template <int D> constexpr int kDqWaves = kWaves[2 + (D == 128)];
+template <int D> constexpr int kDkvWaves = kWaves[4 + (D == 128)];
+
+// ring of a kernel: tiles of two matrices
+template <int D>
+constexpr int kRing = D == 64 ? 3 : 2;
 
 // 4 + 4 consecutive columns of lanes l and l ^ 32 exchanged so that each lane holds 8: register
 // pairs (lo, hi) of column groups 8 a + 4 h (a = 0, 1) -> columns 8 h ... 8 h + 7
@@ -180,9 +212,10 @@ __device__ __forceinline__ int sight(int k0, int i0, int i1, int W, int S) {
 }
 
 template <class E, int D>
-__global__ __launch_bounds__(256) void window_fwd_kernel(WinArgs a, uint16_t* o, uint16_t* rest, float* lse) {
+__global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a, uint16_t* o, uint16_t* rest, float* lse) {
   constexpr int DK = D / 16, DN = D / 32;
-  __shared__ __attribute__((aligned(16))) uint16_t Ks[BN * D], Vs[BN * D];
+  constexpr int NS = kRing<D>;
+  __shared__ __attribute__((aligned(16))) uint16_t ring[NS][2][BN * D];
   const int nqb = (a.Tq + BM - 1) / BM;
   const int item = xcd_remap((int)blockIdx.x, (int)gridDim.x);
   const int qb = item % nqb, bh = item / nqb, b = bh / a.H, hq = bh - b * a.H;
@@ -211,20 +244,18 @@ __global__ __launch_bounds__(256) void window_fwd_kernel(WinArgs a, uint16_t* o,
     const uint16_t* kg = a.k + b * a.k_sb + hk * a.k_sh;
     const uint16_t* vg = a.v + b * a.v_sb + hk * a.v_sh;
     const Tiles tiles(s.st + bt0, s.st + bt1, a.W, a.S);
-    Stage<D> kr, vr;
-    kr.load(kg, a.k_st, tiles.key(0), 0, s.len, tid);
-    vr.load(vg, a.v_st, tiles.key(0), 0, s.len, tid);
+    auto fetch = [&](int it) {
+      fill_tile<D>(kg, a.k_st, tiles.key(it), 0, s.len, ring[it % NS][0], wave, lane);
+      fill_tile<D>(vg, a.v_st, tiles.key(it), 0, s.len, ring[it % NS][1], wave, lane);
+    };
+    for (int it = 0; it < min(NS - 1, tiles.n); ++it) fetch(it);
     for (int it = 0; it < tiles.n; ++it) {
-      __syncthreads();
-      kr.store(Ks, tid);
-      vr.store(Vs, tid);
-      __syncthreads();
-      if (it + 1 < tiles.n) {
-        kr.load(kg, a.k_st, tiles.key(it + 1), 0, s.len, tid);
-        vr.load(vg, a.v_st, tiles.key(it + 1), 0, s.len, tid);
-      }
+      if (it + NS - 1 <= tiles.n) wait_barrier<2 * kFills<D> * (NS - 2)>();
+      else wait_barrier<0>();
+      if (it + NS - 1 < tiles.n) fetch(it + NS - 1);
+      const uint16_t *Ks = ring[it % NS][0], *Vs = ring[it % NS][1];
       if (wt0 > wt1) continue;
-#pragma unroll
+#pragma unroll 1
       for (int sub = 0; sub < 2; ++sub) {
         const int k0 = tiles.key(it) + 32 * sub;
         const int see = sight(k0, s.st + wt0, s.st + wt1, a.W, a.S);
@@ -273,8 +304,7 @@ __global__ __launch_bounds__(256) void window_fwd_kernel(WinArgs a, uint16_t* o,
   const bool some = valid && l > 0.f;
   const int64_t row = (((int64_t)b * a.Tq + t) * a.H + hq) * D;
   put_rows<E, D>(o + row, t < a.Tq, acc, some ? 1.f / l : 0.f, lane, rest ? rest + row : nullptr);
-  if (lse && t < a.Tq && lane < 32)
-    lse[(int64_t)bh * a.Tq + t] = some ? m + log2f(l) : INFINITY;
+  if (lse && lane < 32) lse[(int64_t)bh * nqb * BM + t] = some ? m + log2f(l) : INFINITY;
 }
 
 // dQ, and D of its rows for the dK / dV kernel.  D is formed from o and what o's rounding left off
@@ -282,11 +312,12 @@ __global__ __launch_bounds__(256) void window_fwd_kernel(WinArgs a, uint16_t* o,
 // few keys are seen it is the larger one (a window of 4: 1.8 times the error of a once rounded dq
 // instead of 1.5).
 template <class E, int D>
-__global__ __launch_bounds__(256) void window_dq_kernel(WinArgs a, const uint16_t* o, const uint16_t* rest,
+__global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, const uint16_t* o, const uint16_t* rest,
                                                         const uint16_t* dout, const float* lse, float* dsum, uint16_t* dq,
                                                         float scale) {
   constexpr int DK = D / 16, DN = D / 32;
-  __shared__ __attribute__((aligned(16))) uint16_t Ks[BN * D], Vs[BN * D];
+  constexpr int NS = kRing<D>;
+  __shared__ __attribute__((aligned(16))) uint16_t ring[NS][2][BN * D];
   const int nqb = (a.Tq + BM - 1) / BM;
   const int item = xcd_remap((int)blockIdx.x, (int)gridDim.x);
   const int qb = item % nqb, bh = item / nqb, b = bh / a.H, hq = bh - b * a.H;
@@ -322,24 +353,22 @@ __global__ __launch_bounds__(256) void window_dq_kernel(WinArgs a, const uint16_
       }
     }
     ds = other_half(ds, false);
-    const float ls = valid ? lse[(int64_t)bh * a.Tq + t] : INFINITY;
+    const float ls = lse[(int64_t)bh * nqb * BM + t];
     const uint16_t* kg = a.k + b * a.k_sb + hk * a.k_sh;
     const uint16_t* vg = a.v + b * a.v_sb + hk * a.v_sh;
     const Tiles tiles(s.st + bt0, s.st + bt1, a.W, a.S);
-    Stage<D> kr, vr;
-    kr.load(kg, a.k_st, tiles.key(0), 0, s.len, tid);
-    vr.load(vg, a.v_st, tiles.key(0), 0, s.len, tid);
+    auto fetch = [&](int it) {
+      fill_tile<D>(kg, a.k_st, tiles.key(it), 0, s.len, ring[it % NS][0], wave, lane);
+      fill_tile<D>(vg, a.v_st, tiles.key(it), 0, s.len, ring[it % NS][1], wave, lane);
+    };
+    for (int it = 0; it < min(NS - 1, tiles.n); ++it) fetch(it);
     for (int it = 0; it < tiles.n; ++it) {
-      __syncthreads();
-      kr.store(Ks, tid);
-      vr.store(Vs, tid);
-      __syncthreads();
-      if (it + 1 < tiles.n) {
-        kr.load(kg, a.k_st, tiles.key(it + 1), 0, s.len, tid);
-        vr.load(vg, a.v_st, tiles.key(it + 1), 0, s.len, tid);
-      }
+      if (it + NS - 1 <= tiles.n) wait_barrier<2 * kFills<D> * (NS - 2)>();
+      else wait_barrier<0>();
+      if (it + NS - 1 < tiles.n) fetch(it + NS - 1);
+      const uint16_t *Ks = ring[it % NS][0], *Vs = ring[it % NS][1];
       if (wt0 > wt1) continue;
-#pragma unroll
+#pragma unroll 1
       for (int sub = 0; sub < 2; ++sub) {
         const int k0 = tiles.key(it) + 32 * sub;
         const int see = sight(k0, s.st + wt0, s.st + wt1, a.W, a.S);
@@ -370,136 +399,124 @@ __global__ __launch_bounds__(256) void window_dq_kernel(WinArgs a, const uint16_
     }
   }
   put_rows<E, D>(dq + ((int64_t)bh * a.Tq + t) * D, t < a.Tq, acc, valid ? scale : 0.f, lane);
-  if (t < a.Tq && lane < 32) dsum[(int64_t)bh * a.Tq + t] = valid ? ds : 0.f;
+  if (lane < 32) dsum[(int64_t)bh * nqb * BM + t] = valid ? ds : 0.f;
 }
 
-// dK, dV of 128 keys, 32 a wave.  Items 0 ... nkb - 1 of a key head add up the pairs within the
-// window; behind them come, for each block of keys that holds sinks, `chunks` items that each take
-// `span` queries out of the window of the block's keys: those pairs (j < S, i - j >= W) would
-// otherwise leave a few workgroups with the whole length.  The sums of rows j < S go to `part`
-// [slot][b, hk][S][2][D] in 32 bits (slot 0: the window's), window_sink_kernel adds the slots.
+// dK, dV.  Two kinds of items:
+// near: 128 keys, 32 a wave, with the queries that have them in their window;
+// far: 32 keys, those of sinks, with `span` of the queries that have left their window behind (j < S,
+// i - j >= W) -- pairs that would leave a few workgroups with the whole length.  The four waves take
+// turns at the groups of 32 queries and their sums are added up in the end.
+// The sums of rows j < S go to `part` [slot][b, hk][S][2][D] in 32 bits (slot 0: the near ones, then a
+// slot for each span); window_sink_kernel adds the slots.
 template <class E, int D>
-__global__ __launch_bounds__(256) void window_dkv_kernel(WinArgs a, const uint16_t* dout, const float* lse,
-                                                         const float* dsum, uint16_t* dk, uint16_t* dv,
-                                                         float* part, int chunks, int span, float scale) {
-  constexpr int DK = D / 16, DN = D / 32;
-  __shared__ __attribute__((aligned(16))) uint16_t Qs[BN * D], Os[BN * D];
-  __shared__ __attribute__((aligned(16))) float ls_s[BN], ds_s[BN];
-  const int nkb = (a.Tk + BM - 1) / BM;
-  const int snb = chunks ? (a.S + BM - 1) / BM : 0, items = nkb + snb * chunks;
-  const int item = xcd_remap((int)blockIdx.x, (int)gridDim.x);
-  const int bk = item / items, it0 = item - bk * items, b = bk / a.KV, hk = bk - b * a.KV;
-  const bool far = it0 >= nkb;
-  const int kb = far ? (it0 - nkb) / chunks : it0;
-  const int chunk = far ? (it0 - nkb) % chunks : 0;
-  const Seq s = seq_of(a, b);
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kw = kb * BM + wave * 32, j = kw + (lane & 31);   // the wave's first key, this lane's
-  const bool valid = j < s.len;
-  const int G = a.H / a.KV;
-  constexpr float unshift = 1.f / (1 << E::kShift);           // (elt.h: p is 2^kShift times its value)
-
+struct Dkv {
+  static constexpr int DK = D / 16, DN = D / 32, NS = kRing<D>;
+  struct Lds {
+    uint16_t ring[NS][2][BN * D];
+    float stat[NS][2][BN];                             // log-sums, D
+  };
+  static constexpr float kUnshift = 1.f / (1 << E::kShift);   // (elt.h: p is 2^kShift times its value)
+  const WinArgs& a;
+  const uint16_t* dout;
+  const float *lse, *dsum;
+  Lds& lds;
+  const Seq& s;
+  int b, hk, tq_pad, tid, lane, wave;
+  u32x4 kf[DK], vf[DK];
   f32x16 ak[DN], av[DN];
+
+  // keys kw ... kw + 31 as B operands (zeros behind the sequence), accumulators cleared
+  __device__ __forceinline__ void begin(int kw) {
+    const int j = kw + (lane & 31);
 #pragma unroll
-  for (int dn = 0; dn < DN; ++dn) ak[dn] = av[dn] = zero16();
-  // positions of the queries that this item takes
-  int i0 = kb * BM, i1 = min((int64_t)s.len - 1, (int64_t)kb * BM + BM - 1 + a.W - 1);
-  if (far) {
-    i0 = min((int64_t)s.len, (int64_t)kb * BM + a.W + (int64_t)chunk * span);
-    i1 = min((int64_t)s.len - 1, (int64_t)i0 + span - 1);
-  }
-  const int t0 = max(s.t0, i0 - s.st), t1 = min(s.t1 - 1, i1 - s.st);
-  if (t0 <= t1 && kb * BM < s.len) {
-    u32x4 kf[DK], vf[DK];
+    for (int dn = 0; dn < DN; ++dn) ak[dn] = av[dn] = zero16();
 #pragma unroll
     for (int ks = 0; ks < DK; ++ks) {
       kf[ks] = vf[ks] = u32x4{0, 0, 0, 0};
-      if (valid) {
+      if (j < s.len) {
         const int col = 16 * ks + 8 * (lane >> 5);
         kf[ks] = *(const u32x4*)(a.k + b * a.k_sb + hk * a.k_sh + (int64_t)j * a.k_st + col);
         vf[ks] = *(const u32x4*)(a.v + b * a.v_sb + hk * a.v_sh + (int64_t)j * a.v_st + col);
       }
     }
-    const int tb = t0 & ~(BN - 1), per = (t1 - tb) / BN + 1, n = G * per;
-    Stage<D> qr, dr;
-    float lr = INFINITY, sr = 0.f;
-    auto fetch = [&](int it) {
-      const int hq = hk * G + it / per, row0 = tb + (it % per) * BN;
-      qr.load(a.q + b * a.q_sb + hq * a.q_sh, a.q_st, row0, t0, t1 + 1, tid);
-      dr.load(dout + ((int64_t)b * a.Tq * a.H + hq) * D, (int64_t)a.H * D, row0, t0, t1 + 1, tid);
-      if (tid < BN) {
-        const int t = row0 + tid;
-        const bool ok = t >= t0 && t <= t1;
-        lr = ok ? lse[((int64_t)b * a.H + hq) * a.Tq + t] - E::kShift : INFINITY;
-        sr = ok ? dsum[((int64_t)b * a.H + hq) * a.Tq + t] * unshift : 0.f;
+  }
+
+  // query tile it of `per` tiles a head, the first at row tb
+  __device__ __forceinline__ void fetch(int it, int per, int tb) {
+    const int G = a.H / a.KV, hq = hk * G + it / per, row0 = tb + (it % per) * BN, slot = it % NS;
+    fill_tile<D>(a.q + b * a.q_sb + hq * a.q_sh, a.q_st, row0, s.t0, s.t1, lds.ring[slot][0], wave, lane);
+    fill_tile<D>(dout + ((int64_t)b * a.Tq * a.H + hq) * D, (int64_t)a.H * D, row0, s.t0, s.t1,
+                 lds.ring[slot][1], wave, lane);
+    // (waves 2 and 3 write what waves 0 and 1 do: each has the same number of loads under way)
+    fill4(((wave & 1) ? dsum : lse) + ((int64_t)b * a.H + hq) * tq_pad + row0 + lane, lds.stat[slot][wave & 1]);
+  }
+
+  // queries 32 sub ... of the tile against this wave's keys; ALL: every pair counts
+  template <bool FAR>
+  __device__ __forceinline__ void step(int slot, int sub, int p0, int kw, bool all) {
+    const uint16_t *Qs = lds.ring[slot][0], *Os = lds.ring[slot][1];
+    const float *ls = lds.stat[slot][0], *ds = lds.stat[slot][1];
+    f32x16 x = zero16(), y = zero16();
+#pragma unroll
+    for (int ks = 0; ks < DK; ++ks) {
+      x = E::mfma32(frag<D>(Qs, 32 * sub, ks, lane), kf[ks], x);
+      y = E::mfma32(frag<D>(Os, 32 * sub, ks, lane), vf[ks], y);
+    }
+    const int j = kw + (lane & 31);
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const int q0 = row_of(4 * r4, lane);
+      const f32x4 l4 = *(const f32x4*)(ls + 32 * sub + q0), d4 = *(const f32x4*)(ds + 32 * sub + q0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * r4 + e;
+        float p = __builtin_amdgcn_exp2f(fmaf(x[r], a.c, (float)E::kShift - l4[e]));
+        if (!all) {
+          const int d = p0 + q0 + e - j;               // i - j
+          if (FAR ? (j >= a.S || d < a.W) : (d < 0 || d >= a.W)) p = 0.f;
+        }
+        x[r] = p;
+        y[r] = p * fmaf(d4[e], -kUnshift, y[r] * kUnshift);
       }
-    };
-    fetch(0);
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const u32x4 p = pack<E>(x, st), d = pack<E>(y, st);
+#pragma unroll
+      for (int dn = 0; dn < DN; ++dn) {
+        av[dn] = E::mfma32(frag_t<D>(Os, 32 * sub + 16 * st, dn, lane), p, av[dn]);
+        ak[dn] = E::mfma32(frag_t<D>(Qs, 32 * sub + 16 * st, dn, lane), d, ak[dn]);
+      }
+    }
+  }
+
+  // all tiles of rows [t0, t1) of every query head
+  template <bool FAR>
+  __device__ __forceinline__ void run(int kw, int t0, int t1) {
+    const int tb = t0 & ~(BN - 1), per = (t1 - 1 - tb) / BN + 1, n = per * (a.H / a.KV);
+    for (int it = 0; it < min(NS - 1, n); ++it) fetch(it, per, tb);
     for (int it = 0; it < n; ++it) {
-      __syncthreads();
-      qr.store(Qs, tid);
-      dr.store(Os, tid);
-      if (tid < BN) {
-        ls_s[tid] = lr;
-        ds_s[tid] = sr;
-      }
-      __syncthreads();
-      if (it + 1 < n) fetch(it + 1);
+      if (it + NS - 1 <= n) wait_barrier<(2 * kFills<D> + 1) * (NS - 2)>();
+      else wait_barrier<0>();
+      if (it + NS - 1 < n) fetch(it + NS - 1, per, tb);
       const int row0 = tb + (it % per) * BN;
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        const int p0 = s.st + row0 + 32 * sub;                // position of the group's first query
-        bool all;
-        if (far) {                                            // pairs j < S, i - j >= W
-          if (kw >= a.S || p0 + 31 - kw < a.W) continue;
-          all = kw + 31 < a.S && p0 - (kw + 31) >= a.W;
-        } else {                                              // pairs j <= i, i - j < W
+      if (FAR) {
+        if ((it & 1) != (wave >> 1)) continue;
+        const int sub = wave & 1, p0 = s.st + row0 + 32 * sub;
+        if (p0 + 31 - kw >= a.W) step<true>(it % NS, sub, p0, kw, kw + 31 < a.S && p0 - (kw + 31) >= a.W);
+      } else {
+#pragma unroll 1
+        for (int sub = 0; sub < 2; ++sub) {
+          const int p0 = s.st + row0 + 32 * sub;
           if (p0 + 31 < kw || p0 - (kw + 31) >= a.W) continue;
-          all = p0 >= kw + 31 && p0 + 31 - kw < a.W;
-        }
-        f32x16 x = zero16(), y = zero16();
-#pragma unroll
-        for (int ks = 0; ks < DK; ++ks) {
-          x = E::mfma32(frag<D>(Qs, 32 * sub, ks, lane), kf[ks], x);
-          y = E::mfma32(frag<D>(Os, 32 * sub, ks, lane), vf[ks], y);
-        }
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const int q0 = 32 * sub + row_of(4 * r4, lane);
-          const f32x4 l4 = *(const f32x4*)(ls_s + q0), d4 = *(const f32x4*)(ds_s + q0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * r4 + e;
-            float p = __builtin_amdgcn_exp2f(fmaf(x[r], a.c, -l4[e]));
-            if (!all) {
-              const int d = s.st + row0 + q0 + e - j;         // i - j
-              if (far ? (j >= a.S || d < a.W) : (d < 0 || d >= a.W)) p = 0.f;
-            }
-            x[r] = p;
-            y[r] = p * fmaf(y[r], unshift, -d4[e]);
-          }
-        }
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const u32x4 p = pack<E>(x, st), d = pack<E>(y, st);
-#pragma unroll
-          for (int dn = 0; dn < DN; ++dn) {
-            av[dn] = E::mfma32(frag_t<D>(Os, 32 * sub + 16 * st, dn, lane), p, av[dn]);
-            ak[dn] = E::mfma32(frag_t<D>(Qs, 32 * sub + 16 * st, dn, lane), d, ak[dn]);
-          }
+          step<false>(it % NS, sub, p0, kw, p0 >= kw + 31 && p0 + 31 - kw < a.W);
         }
       }
     }
   }
-  const bool sink = chunks && j < a.S;
-  if (!far) {
-    const int64_t row = ((int64_t)bk * a.Tk + j) * D;
-    put_rows<E, D>(dk + row, j < a.Tk && !sink, ak, scale, lane);
-    put_rows<E, D>(dv + row, j < a.Tk && !sink, av, unshift, lane);
-  }
-  if (sink && j < a.Tk) {
-    const int slot = far ? 1 + chunk : 0;
-    float* dst = part + (((int64_t)slot * a.B * a.KV + bk) * a.S + j) * 2 * D;
+
+  __device__ __forceinline__ void put_part(float* dst) const {
 #pragma unroll
     for (int dn = 0; dn < DN; ++dn)
 #pragma unroll
@@ -509,6 +526,62 @@ __global__ __launch_bounds__(256) void window_dkv_kernel(WinArgs a, const uint16
         *(f32x4*)(dst + D + col) = f32x4{av[dn][4 * r4], av[dn][4 * r4 + 1], av[dn][4 * r4 + 2], av[dn][4 * r4 + 3]};
       }
   }
+
+  // x of the four waves added up in wave 0, in their order
+  __device__ __forceinline__ void join(f32x16 (&x)[DN]) {
+    float* buf = (float*)&lds;                         // 3 waves, 16 DN registers, 64 lanes
+    __syncthreads();
+    if (wave)
+#pragma unroll
+      for (int dn = 0; dn < DN; ++dn)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) buf[(((wave - 1) * DN + dn) * 16 + r) * 64 + lane] = x[dn][r];
+    __syncthreads();
+    if (!wave)
+      for (int w = 0; w < 3; ++w)
+#pragma unroll
+        for (int dn = 0; dn < DN; ++dn)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[dn][r] += buf[((w * DN + dn) * 16 + r) * 64 + lane];
+  }
+};
+
+template <class E, int D>
+__global__ __launch_bounds__(256, kDkvWaves<D>) void window_dkv_kernel(WinArgs a, const uint16_t* dout, const float* lse,
+                                                         const float* dsum, uint16_t* dk, uint16_t* dv,
+                                                         float* part, int spans, int span, float scale) {
+  using K = Dkv<E, D>;
+  static_assert(sizeof(typename K::Lds) >= 3 * 64 * D / 2 * 4, "room to join the waves");
+  __shared__ __attribute__((aligned(16))) typename K::Lds lds;
+  const int nkb = (a.Tk + BM - 1) / BM;
+  const int nst = spans ? (a.S + 31) / 32 : 0, items = nkb + nst * spans;
+  const int item = xcd_remap((int)blockIdx.x, (int)gridDim.x);
+  const int bk = item / items, it0 = item - bk * items, b = bk / a.KV, hk = bk - b * a.KV;
+  const Seq s = seq_of(a, b);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  K k{a, dout, lse, dsum, lds, s, b, hk, (a.Tq + BM - 1) / BM * BM, tid, lane, wave};
+  if (it0 < nst * spans) {
+    const int c = it0 % spans, kw = it0 / spans * 32, j = kw + (lane & 31);
+    const int t0 = (int)max((int64_t)max(s.t0, c * span), (int64_t)a.W + kw - s.st);
+    const int t1 = (int)min((int64_t)s.t1, (int64_t)(c + 1) * span);
+    k.begin(kw);
+    if (t0 < t1 && kw < s.len) k.template run<true>(kw, t0, t1);
+    k.join(k.ak);
+    k.join(k.av);
+    if (!wave && j < a.S) k.put_part(part + (((int64_t)(1 + c) * a.B * a.KV + bk) * a.S + j) * 2 * D);
+    return;
+  }
+  const int kb = it0 - nst * spans, kw = kb * BM + wave * 32, j = kw + (lane & 31);
+  // positions [kb BM, last key + W)
+  const int t0 = max(s.t0, kb * BM - s.st);
+  const int t1 = (int)min((int64_t)s.t1, (int64_t)kb * BM + BM - 1 + a.W - s.st);
+  k.begin(kw);
+  if (t0 < t1 && kb * BM < s.len) k.template run<false>(kw, t0, t1);
+  const bool sink = spans && j < a.S;
+  const int64_t row = ((int64_t)bk * a.Tk + j) * D;
+  put_rows<E, D>(dk + row, j < a.Tk && !sink, k.ak, scale, lane);
+  put_rows<E, D>(dv + row, j < a.Tk && !sink, k.av, K::kUnshift, lane);
+  if (sink) k.put_part(part + ((int64_t)bk * a.S + j) * 2 * D);
 }
 
 // dk, dv rows j < min(S, Tk) from the slots of window_dkv_kernel, in their order
@@ -541,22 +614,22 @@ int fwd(const WinArgs& a, void* o, void* rest, void* lse, hipStream_t st) {
 
 template <class E, int D>
 int bwd(const WinArgs& a, const void* o, const void* rest, const void* dout, const void* lse, void* dsum, void* dq, void* dk,
-        void* dv, void* part, int chunks, int span, float scale, hipStream_t st) {
+        void* dv, void* part, int spans, int span, float scale, hipStream_t st) {
   const int64_t n = (int64_t)((a.Tq + BM - 1) / BM) * a.B * a.H;
-  const int64_t nk = ((int64_t)(a.Tk + BM - 1) / BM + (chunks ? (int64_t)((a.S + BM - 1) / BM) * chunks : 0)) *
+  const int64_t nk = ((int64_t)(a.Tk + BM - 1) / BM + (int64_t)((a.S + 31) / 32) * spans) *
                      a.B * a.KV;
   if (n >= (1ll << 31) || nk >= (1ll << 31)) return 1;
   hipLaunchKernelGGL((window_dq_kernel<E, D>), dim3((unsigned)n), dim3(256), 0, st, a, (const uint16_t*)o,
                      (const uint16_t*)rest, (const uint16_t*)dout, (const float*)lse, (float*)dsum, (uint16_t*)dq,
                      scale);
   hipLaunchKernelGGL((window_dkv_kernel<E, D>), dim3((unsigned)nk), dim3(256), 0, st, a, (const uint16_t*)dout,
-                     (const float*)lse, (const float*)dsum, (uint16_t*)dk, (uint16_t*)dv, (float*)part, chunks,
+                     (const float*)lse, (const float*)dsum, (uint16_t*)dk, (uint16_t*)dv, (float*)part, spans,
                      span, scale);
-  if (chunks) {
+  if (spans) {
     const int64_t threads = (int64_t)a.B * a.KV * a.S * 2 * (D / 4);
     if ((threads + 255) / 256 >= (1ll << 31)) return 1;
     hipLaunchKernelGGL((window_sink_kernel<E, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st,
-                       (const float*)part, 1 + chunks, a.B * a.KV, a.S, a.Tk, (uint16_t*)dk, (uint16_t*)dv, scale);
+                       (const float*)part, 1 + spans, a.B * a.KV, a.S, a.Tk, (uint16_t*)dk, (uint16_t*)dv, scale);
   }
   return (int)hipGetLastError();
 }
@@ -579,8 +652,8 @@ WinArgs args(const void* q, const void* k, const void* v, const int64_t* s, cons
 extern "C" {
 
 // dtype 0: bf16, 1: fp16.  strides: (batch, head, row) of q, k, v in elements; rows are contiguous
-// and 16-byte aligned (checked by the caller).  o, rest: [B][Tq][H][D]; lse: [B][H][Tq]; rest and lse
-// (for the backward) or null.
+// and 16-byte aligned (checked by the caller).  o, rest: [B][Tq][H][D]; lse: [B][H][Tq rounded
+// up to 128]; rest and lse (for the backward) or null.
 int mopt_window_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* start,
                     const void* lengths, int start0, void* o, void* rest, void* lse, int B, int H, int KV, int Tq, int Tk,
                     int D, int W, int S, float scale, int dtype, void* stream) {
@@ -591,22 +664,22 @@ int mopt_window_fwd(const void* q, const void* k, const void* v, const int64_t* 
   return D == 64 ? fwd<Fp16, 64>(a, o, rest, lse, st) : fwd<Fp16, 128>(a, o, rest, lse, st);
 }
 
-// dq [B][H][Tq][D], dk, dv [B][KV][Tk][D]; dsum: [B][H][Tq] floats of workspace; part: workspace of
-// (1 + chunks) B KV S 2 D floats, chunks * span queries being all that the first sink sees out of
-// its window (chunks 0: none does)
+// dq [B][H][Tq][D], dk, dv [B][KV][Tk][D]; dsum: floats of workspace; part: workspace of
+// (1 + spans) B KV S 2 D floats, spans * span >= Tq (spans 0: no sink is seen out of its window);
+// lse, dsum: rows of Tq rounded up to 128
 int mopt_window_bwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* start,
                     const void* lengths, int start0, const void* o, const void* rest, const void* dout, const void* lse, void* dsum,
-                    void* dq, void* dk, void* dv, void* part, int chunks, int span, int B, int H, int KV, int Tq,
+                    void* dq, void* dk, void* dv, void* part, int spans, int span, int B, int H, int KV, int Tq,
                     int Tk, int D, int W, int S, float scale, int dtype, void* stream) {
   const WinArgs a = args(q, k, v, strides, start, lengths, start0, B, H, KV, Tq, Tk, W, S, scale);
-  if (!good(a, D) || chunks < 0 || (chunks && (span <= 0 || !part || S == 0))) return 1;
-  if ((int64_t)chunks * span < (S ? (int64_t)Tk - W : 0)) return 1;
+  if (!good(a, D) || spans < 0 || span <= 0 || span % BN || (spans && (!part || S == 0))) return 1;
+  if (S && Tk > W && (int64_t)spans * span < Tq) return 1;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0)
-    return D == 64 ? bwd<Bf16, 64>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, chunks, span, scale, st)
-                   : bwd<Bf16, 128>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, chunks, span, scale, st);
-  return D == 64 ? bwd<Fp16, 64>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, chunks, span, scale, st)
-                 : bwd<Fp16, 128>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, chunks, span, scale, st);
+    return D == 64 ? bwd<Bf16, 64>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, spans, span, scale, st)
+                   : bwd<Bf16, 128>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, spans, span, scale, st);
+  return D == 64 ? bwd<Fp16, 64>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, spans, span, scale, st)
+                 : bwd<Fp16, 128>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, spans, span, scale, st);
 }
 
 }  // extern "C"

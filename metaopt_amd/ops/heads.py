@@ -286,7 +286,7 @@ def window_attention_ref(q, k, v, window=None, sinks=0, scale=None, start=None, 
 
 
 #: queries of one out-of-window item of the dK / dV kernel (csrc/lm_window.hip)
-_SINK_SPAN = 1024
+_SINK_SPAN = 512
 
 
 def _geometry(q, k, v):
@@ -298,7 +298,7 @@ def _window_fwd(q, k, v, window, sinks, scale, start, start0, lengths, train):
     KV, Tk = k.shape[1], k.shape[2]
     o = torch.empty(B * Tq, H * D, dtype=q.dtype, device=q.device)
     # for the backward: the log-sums and what the rounding of o left off
-    lse = torch.empty(B, H, Tq, dtype=torch.float32, device=q.device) if train else None
+    lse = torch.empty(B, H, -(-Tq // 128) * 128, dtype=torch.float32, device=q.device) if train else None
     rest = torch.empty_like(o) if train else None
     if o.numel() and Tk:
         _call(q, "mopt_window_fwd", _p(q), _p(k), _p(v), _geometry(q, k, v), _p(start), _p(lengths),
@@ -329,13 +329,12 @@ class _WindowAttention(torch.autograd.Function):
         if not o.numel() or not Tk:
             return (dq.zero_(), dk.zero_(), dv.zero_()) + (None,) * 6
         dsum = torch.empty_like(lse)
-        beyond = Tk - window if sinks else 0
-        chunks = -(-beyond // _SINK_SPAN) if beyond > 0 else 0
-        part = torch.empty((1 + chunks) * B * KV * sinks * 2 * D if chunks else 0,
+        spans = -(-Tq // _SINK_SPAN) if sinks and Tk > window else 0
+        part = torch.empty((1 + spans) * B * KV * sinks * 2 * D if spans else 0,
                            dtype=torch.float32, device=q.device)
         _call(q, "mopt_window_bwd", _p(q), _p(k), _p(v), _geometry(q, k, v), _p(start), _p(lengths),
               start0, _p(o), _p(rest), _p(_dense16(do)), _p(lse), _p(dsum), _p(dq), _p(dk), _p(dv), _p(part),
-              chunks, _SINK_SPAN, B, H, KV, Tq, Tk, D, window, sinks, scale, _TYPES[q.dtype])
+              spans, _SINK_SPAN, B, H, KV, Tq, Tk, D, window, sinks, scale, _TYPES[q.dtype])
         return (dq, dk, dv) + (None,) * 6
 
 
