@@ -54,7 +54,7 @@ __device__ __forceinline__ int swz(int r) {
   return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 2) << 1) | ((r >> 2) & 3);
 }
 template <int D>
-__device__ __forceinline__ int at(int r, int c) {      // element offset of (row, column)
+__device__ __forceinline__ int lds_off(int r, int c) {      // element offset of (row, column)
   return r * D + (((c >> 3) ^ swz<D>(r)) << 3) + (c & 7);
 }
 
@@ -62,20 +62,33 @@ __device__ __forceinline__ u32x4 lds16(const uint16_t* p) { return *(const u32x4
 
 __device__ __forceinline__ int swap23(int r) { return (r & 19) | ((r & 4) << 1) | ((r & 8) >> 1); }
 
-// A operand of rows [r0, r0 + 32) in the exchanged order, columns 16 ks ... + 15
-template <int D>
-__device__ __forceinline__ u32x4 frag(const uint16_t* s, int r0, int ks, int lane) {
-  return lds16(s + at<D>(r0 + swap23(lane & 31), 16 * ks + 8 * (lane >> 5)));
-}
+typedef __attribute__((address_space(3))) void lds_void;
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)((lds_void*)p); }
 
-// A operand of the transpose: rows = columns [32 dn, 32 dn + 32) of the tile, k = rows r0 ... + 15
+// Fragments of a tile at LDS address `tile` (a multiple of 256).  A lane's place in the tile is kept
+// in one register; columns change it by an exclusive or, rows by an offset of the instruction.
 template <int D>
-__device__ __forceinline__ u32x4 frag_t(const uint16_t* s, int r0, int dn, int lane) {
-  const int g = lane >> 4, i = lane & 15;
-  const int row = r0 + 8 * (g >> 1) + (i >> 2), col = 32 * dn + 16 * (g & 1) + 4 * (i & 3);
-  return __builtin_bit_cast(u32x4, cat_frag(lds_tr4((const bf16_t*)s + at<D>(row, col)),
-                                            lds_tr4((const bf16_t*)s + at<D>(row + 4, col))));
-}
+struct Place {
+  uint32_t f, t;
+  __device__ __forceinline__ explicit Place(int lane) {
+    const int r = swap23(lane & 31), g = lane >> 4, i = lane & 15, q = 8 * (g >> 1) + (i >> 2);
+    f = r * D * 2 + (((lane >> 5) ^ swz<D>(r)) << 4);
+    t = q * D * 2 + (((2 * (g & 1) + ((i & 3) >> 1)) ^ swz<D>(q)) << 4) + (i & 1) * 8;
+  }
+  // A operand of rows [r0, r0 + 32) (r0 a multiple of 32) in the exchanged order, columns 16 ks ...
+  __device__ __forceinline__ u32x4 frag(uint32_t tile, int r0, int ks) const {
+    typedef __attribute__((address_space(3))) const u32x4 vec;
+    return *(vec*)(uintptr_t)(((tile + f) ^ (ks << 5)) + r0 * D * 2);
+  }
+  // A operand of the transpose: rows = columns [32 dn, 32 dn + 32) of the tile, k = rows r0 ... + 15
+  // (r0 a multiple of 16); rows 4 further have bit 0 of their exchange turned
+  __device__ __forceinline__ u32x4 frag_t(uint32_t tile, int r0, int dn) const {
+    const uint32_t p = (tile + t) ^ (dn << 6);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(p + r0 * D * 2));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((p ^ 16) + (r0 + 4) * D * 2));
+    return __builtin_bit_cast(u32x4, cat_frag(lo, hi));
+  }
+};
 
 // registers 8 s ... 8 s + 7 of an accumulator as the B operand of step s
 template <class E>
@@ -106,16 +119,22 @@ __device__ __forceinline__ f32x16 zero16() {
 // tile_wait waits for those of the next tile itself.  Rows outside [lo, hi) are read as the nearest
 // row inside (values of the sequence, finite as the others; the masks leave them out): what padding
 // holds is never read.
-typedef __attribute__((address_space(3))) void lds_void;
-
-__device__ __forceinline__ uint32_t lds_at(const void* p) {
-  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)((lds_void*)p));
+__device__ __forceinline__ uint32_t lds_at(const void* p) { return __builtin_amdgcn_readfirstlane(lds_addr(p)); }
+// base: the same for the whole wave; off: bytes, each lane's own.  (m0 is read a wait state after it is set.)
+__device__ __forceinline__ const char* scalar(const void* p) {
+  // (readfirstlane gives an int: the low half must not be extended by its sign)
+  const uint64_t v = (uint64_t)p;
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (const char*)((uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ void fill16(const void* src, const void* dst) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_at(dst)) : "memory", "m0");
+__device__ __forceinline__ void fill16(const char* base, uint32_t off, const void* dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_at(dst))
+               : "memory");
 }
-__device__ __forceinline__ void fill4(const void* src, const void* dst) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds_at(dst)) : "memory", "m0");
+__device__ __forceinline__ void fill4(const char* base, uint32_t off, const void* dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds_at(dst))
+               : "memory");
 }
 
 // until at most N of this wave's loads are under way, then until every wave is there
@@ -124,33 +143,28 @@ __device__ __forceinline__ void wait_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <int D>
-constexpr int kFills = BN * D * 2 / 1024 / 4;          // 1 KB fills of a tile by each of 4 waves
+template <int D, int ROWS = BN>
+constexpr int kFills = ROWS * D * 2 / 1024 / 4;        // 1 KB fills of a tile by each of 4 waves
 
-template <int D>
+template <int D, int ROWS = BN>
 __device__ __forceinline__ void fill_tile(const uint16_t* g, int64_t ld, int row0, int lo, int hi, uint16_t* img,
                                           int wave, int lane) {
   constexpr int CH = D / 8, PER = 64 / CH;             // chunks of a row, rows of a fill
+  const char* base = scalar(g + row0 * ld);
+  const int first = lo - row0, last = hi - 1 - row0;   // (last >= 0: a tile starts inside)
 #pragma unroll
-  for (int j = 0; j < kFills<D>; ++j) {
-    const int blk = wave * kFills<D> + j, r = blk * PER + lane / CH, c = (lane % CH) ^ swz<D>(r);
-    const int row = max(lo, min(hi - 1, row0 + r));
-    fill16(g + row * ld + c * 8, img + blk * 512);
+  for (int j = 0; j < kFills<D, ROWS>; ++j) {
+    const int blk = wave * kFills<D, ROWS> + j, r = blk * PER + lane / CH, c = (lane % CH) ^ swz<D>(r);
+    fill16(base, (uint32_t)max(first, min(last, r)) * ((uint32_t)ld * 2) + c * 16, img + blk * 512);
   }
 }
 
-// waves a SIMD: the registers that a kernel may use (512 / waves)
-#ifndef MOPT_WINDOW_WAVES
-#define MOPT_WINDOW_WAVES 3, 2, 3, 2, 3, 2
-#endif
-constexpr int kWaves[6] = {MOPT_WINDOW_WAVES};
-template <int D> constexpr int kFwdWaves = kWaves[D == 128];
-template <int D> constexpr int kDqWaves = kWaves[2 + (D == 128)];
-template <int D> constexpr int kDkvWaves = kWaves[4 + (D == 128)];
-
-// ring of a kernel: tiles of two matrices
-template <int D>
-constexpr int kRing = D == 64 ? 3 : 2;
+// waves a SIMD (registers: 512 / waves) and ring of a kernel (tiles of two matrices)
+template <int D> constexpr int kFwdWaves = D == 64 ? 4 : 2;
+template <int D> constexpr int kDqWaves = D == 64 ? 3 : 2;
+template <int D> constexpr int kDkvWaves = D == 64 ? 3 : 2;
+template <int D> constexpr int kFwdRing = 2;
+template <int D> constexpr int kBwdRing = D == 64 ? 3 : 2;
 
 // 4 + 4 consecutive columns of lanes l and l ^ 32 exchanged so that each lane holds 8: register
 // pairs (lo, hi) of column groups 8 a + 4 h (a = 0, 1) -> columns 8 h ... 8 h + 7
@@ -163,33 +177,60 @@ __device__ __forceinline__ u32x4 join_halves(const float* a0, const float* a1) {
   return u32x4{p[0], q[0], p[1], q[1]};
 }
 
-// rows = lanes (l & 31), columns 32 dn + ...: store an accumulator [D][32] transposed into a row;
-// with `rest`, what its rounding left off goes there, rounded
-template <class E, int D>
-__device__ __forceinline__ void put_rows(uint16_t* row, bool ok, const f32x16 (&acc)[D / 32], float f,
-                                         int lane, uint16_t* rest = nullptr) {
+// ------------------------------------------------------------------------------------ a wave's rows
+// 32 rows of D values between memory and a wave's fragments go through an image in LDS that is the
+// wave's own, so that memory is read and written in whole rows: fragments straight from memory touch
+// 32 lines for 32 bytes each (125M step, dQ without any products: 94 us so, with a window of 1).
+template <int D>
+struct Rows {
+  static constexpr int CH = D / 8, PER = 64 / CH, N = 32 / PER;   // chunks a row, rows a pass, passes
+  static constexpr int SIZE = 32 * D;                              // elements of an image
+
+  // rows row0 ... of a matrix; those outside [lo, hi) as the nearest inside
+  static __device__ __forceinline__ void fill(const uint16_t* g, int64_t ld, int row0, int lo, int hi,
+                                              uint16_t* img, int lane) {
+    row0 = min(row0, hi - 1);                          // (a wave without a row inside)
+    const char* base = scalar(g + row0 * ld);
+    const int first = lo - row0, last = hi - 1 - row0;
 #pragma unroll
-  for (int dn = 0; dn < D / 32; ++dn)
+    for (int j = 0; j < N; ++j) {
+      const int r = j * PER + lane / CH, c = (lane % CH) ^ swz<D>(r);
+      fill16(base, (uint32_t)max(first, min(last, r)) * ((uint32_t)ld * 2) + c * 16, img + j * 512);
+    }
+  }
+  // the B operand of step ks: this lane's row, columns 16 ks + 8 (l >> 5) ...
+  static __device__ __forceinline__ void read(const uint16_t* img, u32x4 (&f)[D / 16], int lane) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      float x[2][4];
+    for (int ks = 0; ks < D / 16; ++ks) f[ks] = lds16(img + lds_off<D>(lane & 31, 16 * ks + 8 * (lane >> 5)));
+  }
+  // acc * f, rounded, into rows row0 ... < hi of a matrix; with REST, what the rounding left off
+  template <class E, bool REST>
+  static __device__ __forceinline__ void put(const f32x16 (&acc)[D / 32], float f, uint16_t* g, int64_t ld,
+                                             int row0, int lo, int hi, uint16_t* img, int lane) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[0][j] = acc[dn][8 * a + j] * f;
-        x[1][j] = acc[dn][8 * a + 4 + j] * f;
-      }
-      const u32x4 w = join_halves<E>(x[0], x[1]);
-      if (ok) *(u32x4*)(row + 32 * dn + 16 * a + 8 * (lane >> 5)) = w;
-      if (rest) {
+    for (int dn = 0; dn < D / 32; ++dn)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        float x[2][4];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float v = x[j >> 2][j & 3];
-          x[j >> 2][j & 3] = v - E::up(E::pack2(v, v) & 0xFFFF);
+          const float v = acc[dn][8 * a + j] * f;
+          x[j >> 2][j & 3] = REST ? v - E::up(E::pack2(v, v) & 0xFFFF) : v;
         }
-        const u32x4 lo = join_halves<E>(x[0], x[1]);
-        if (ok) *(u32x4*)(rest + 32 * dn + 16 * a + 8 * (lane >> 5)) = lo;
+        *(u32x4*)(img + lds_off<D>(lane & 31, 32 * dn + 16 * a + 8 * (lane >> 5))) = join_halves<E>(x[0], x[1]);
       }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int r = j * PER + lane / CH, c = lane % CH, row = row0 + r;
+      const u32x4 w = lds16(img + lds_off<D>(r, c * 8));
+      if (row >= lo && row < hi) *(u32x4*)(g + row * ld + c * 8) = w;
     }
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void wait_own() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 // The key tiles of queries [i0, i1] (positions): first the sink tiles in front of the window,
@@ -212,48 +253,50 @@ __device__ __forceinline__ int sight(int k0, int i0, int i1, int W, int S) {
 }
 
 template <class E, int D>
-__global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a, uint16_t* o, uint16_t* rest, float* lse) {
-  constexpr int DK = D / 16, DN = D / 32;
-  constexpr int NS = kRing<D>;
-  __shared__ __attribute__((aligned(16))) uint16_t ring[NS][2][BN * D];
+__global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a, uint16_t* o, uint16_t* rest,
+                                                                       float* lse) {
+  constexpr int DK = D / 16, DN = D / 32, NS = kFwdRing<D>;
+  __shared__ __attribute__((aligned(256))) uint16_t ring[NS][2][BN * D];
   const int nqb = (a.Tq + BM - 1) / BM;
   const int item = xcd_remap((int)blockIdx.x, (int)gridDim.x);
   const int qb = item % nqb, bh = item / nqb, b = bh / a.H, hq = bh - b * a.H;
   const int hk = hq / (a.H / a.KV);
   const Seq s = seq_of(a, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int t = qb * BM + wave * 32 + (lane & 31);        // this lane's query
+  const int tw = qb * BM + wave * 32, t = tw + (lane & 31);   // the wave's first query, this lane's
   const bool valid = t >= s.t0 && t < s.t1;
   const int i = s.st + t;
   // valid queries of the block and of the wave
   const int bt0 = max(s.t0, qb * BM), bt1 = min(s.t1, qb * BM + BM) - 1;
-  const int wt0 = max(s.t0, qb * BM + wave * 32), wt1 = min(s.t1, qb * BM + wave * 32 + 32) - 1;
+  const int wt0 = max(s.t0, tw), wt1 = min(s.t1, tw + 32) - 1;
 
+  const Place<D> at(lane);
   f32x16 acc[DN];
 #pragma unroll
   for (int dn = 0; dn < DN; ++dn) acc[dn] = zero16();
   float m = -3e38f, l = 0.f;
+  // the wave's image, in the slot that is filled last
+  uint16_t* img = ring[0][0] + wave * Rows<D>::SIZE;
   if (bt0 <= bt1) {
-    u32x4 qf[DK];
-#pragma unroll
-    for (int ks = 0; ks < DK; ++ks) {
-      qf[ks] = u32x4{0, 0, 0, 0};
-      if (valid)
-        qf[ks] = *(const u32x4*)(a.q + b * a.q_sb + hq * a.q_sh + (int64_t)t * a.q_st + 16 * ks + 8 * (lane >> 5));
-    }
     const uint16_t* kg = a.k + b * a.k_sb + hk * a.k_sh;
     const uint16_t* vg = a.v + b * a.v_sb + hk * a.v_sh;
     const Tiles tiles(s.st + bt0, s.st + bt1, a.W, a.S);
+    // (slot of tile 0: 1)
     auto fetch = [&](int it) {
-      fill_tile<D>(kg, a.k_st, tiles.key(it), 0, s.len, ring[it % NS][0], wave, lane);
-      fill_tile<D>(vg, a.v_st, tiles.key(it), 0, s.len, ring[it % NS][1], wave, lane);
+      fill_tile<D>(kg, a.k_st, tiles.key(it), 0, s.len, ring[(it + 1) % NS][0], wave, lane);
+      fill_tile<D>(vg, a.v_st, tiles.key(it), 0, s.len, ring[(it + 1) % NS][1], wave, lane);
     };
+    Rows<D>::fill(a.q + b * a.q_sb + hq * a.q_sh, a.q_st, tw, s.t0, s.t1, img, lane);
     for (int it = 0; it < min(NS - 1, tiles.n); ++it) fetch(it);
+    if (tiles.n >= NS - 1) wait_own<2 * kFills<D> * (NS - 1)>();
+    else wait_own<0>();
+    u32x4 qf[DK];
+    Rows<D>::read(img, qf, lane);
     for (int it = 0; it < tiles.n; ++it) {
       if (it + NS - 1 <= tiles.n) wait_barrier<2 * kFills<D> * (NS - 2)>();
       else wait_barrier<0>();
       if (it + NS - 1 < tiles.n) fetch(it + NS - 1);
-      const uint16_t *Ks = ring[it % NS][0], *Vs = ring[it % NS][1];
+      const uint32_t Ks = lds_at(ring[(it + 1) % NS][0]), Vs = lds_at(ring[(it + 1) % NS][1]);
       if (wt0 > wt1) continue;
 #pragma unroll 1
       for (int sub = 0; sub < 2; ++sub) {
@@ -262,12 +305,17 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
         if (see == 0) continue;
         f32x16 x = zero16();
 #pragma unroll
-        for (int ks = 0; ks < DK; ++ks) x = E::mfma32(frag<D>(Ks, 32 * sub, ks, lane), qf[ks], x);
+        for (int ks = 0; ks < DK; ++ks) x = E::mfma32(at.frag(Ks + sub * 64 * D, 0, ks), qf[ks], x);
         if (see == 1) {
+          const int d0 = i - k0 - 8 * (lane >> 5);
+          if (k0 >= a.S) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int j = k0 + row_of(r, lane);
-            if (j > i || (i - j >= a.W && j >= a.S)) x[r] = -INFINITY;
+            for (int r = 0; r < 16; ++r) x[r] = (uint32_t)(d0 - row_of(r, 0)) < (uint32_t)a.W ? x[r] : -INFINITY;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              x[r] = (uint32_t)(d0 - row_of(r, 0)) < (k0 + row_of(r, lane) < a.S ? 1u << 31 : (uint32_t)a.W)
+                         ? x[r] : -INFINITY;
           }
         }
         float mx = x[0];
@@ -295,15 +343,18 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
           const u32x4 p = pack<E>(x, st);
 #pragma unroll
           for (int dn = 0; dn < DN; ++dn)
-            acc[dn] = E::mfma32(frag_t<D>(Vs, 32 * sub + 16 * st, dn, lane), p, acc[dn]);
+            acc[dn] = E::mfma32(at.frag_t(Vs + sub * 64 * D, 16 * st, dn), p, acc[dn]);
         }
       }
     }
   }
   l = other_half(l, false);
   const bool some = valid && l > 0.f;
-  const int64_t row = (((int64_t)b * a.Tq + t) * a.H + hq) * D;
-  put_rows<E, D>(o + row, t < a.Tq, acc, some ? 1.f / l : 0.f, lane, rest ? rest + row : nullptr);
+  const float f = some ? 1.f / l : 0.f;
+  const int64_t ld = (int64_t)a.H * D, base = ((int64_t)b * a.Tq * a.H + hq) * D;
+  __syncthreads();                                     // (the tiles have been read)
+  Rows<D>::template put<E, false>(acc, f, o + base, ld, tw, 0, a.Tq, img, lane);
+  if (rest) Rows<D>::template put<E, true>(acc, f, rest + base, ld, tw, 0, a.Tq, img, lane);
   if (lse && lane < 32) lse[(int64_t)bh * nqb * BM + t] = some ? m + log2f(l) : INFINITY;
 }
 
@@ -312,61 +363,75 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
 // few keys are seen it is the larger one (a window of 4: 1.8 times the error of a once rounded dq
 // instead of 1.5).
 template <class E, int D>
-__global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, const uint16_t* o, const uint16_t* rest,
-                                                        const uint16_t* dout, const float* lse, float* dsum, uint16_t* dq,
-                                                        float scale) {
-  constexpr int DK = D / 16, DN = D / 32;
-  constexpr int NS = kRing<D>;
-  __shared__ __attribute__((aligned(16))) uint16_t ring[NS][2][BN * D];
+__global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, const uint16_t* o,
+                                                                     const uint16_t* rest, const uint16_t* dout,
+                                                                     const float* lse, float* dsum, uint16_t* dq,
+                                                                     float scale) {
+  constexpr int DK = D / 16, DN = D / 32, NS = kBwdRing<D>, CH = Rows<D>::CH, PER = Rows<D>::PER;
+  __shared__ __attribute__((aligned(256))) uint16_t ring[NS][2][BN * D];
+  __shared__ float ds_s[BM];
   const int nqb = (a.Tq + BM - 1) / BM;
   const int item = xcd_remap((int)blockIdx.x, (int)gridDim.x);
   const int qb = item % nqb, bh = item / nqb, b = bh / a.H, hq = bh - b * a.H;
   const int hk = hq / (a.H / a.KV);
   const Seq s = seq_of(a, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int t = qb * BM + wave * 32 + (lane & 31);
+  const int tw = qb * BM + wave * 32, t = tw + (lane & 31);
   const bool valid = t >= s.t0 && t < s.t1;
   const int i = s.st + t;
   const int bt0 = max(s.t0, qb * BM), bt1 = min(s.t1, qb * BM + BM) - 1;
-  const int wt0 = max(s.t0, qb * BM + wave * 32), wt1 = min(s.t1, qb * BM + wave * 32 + 32) - 1;
+  const int wt0 = max(s.t0, tw), wt1 = min(s.t1, tw + 32) - 1;
 
+  const Place<D> at(lane);
   f32x16 acc[DN];
 #pragma unroll
   for (int dn = 0; dn < DN; ++dn) acc[dn] = zero16();
   float ds = 0.f;
+  uint16_t* img = ring[0][0] + wave * Rows<D>::SIZE;
   if (bt0 <= bt1) {
-    u32x4 qf[DK], df[DK];
-    const int64_t row = (((int64_t)b * a.Tq + t) * a.H + hq) * D;
-#pragma unroll
-    for (int ks = 0; ks < DK; ++ks) {
-      qf[ks] = df[ks] = u32x4{0, 0, 0, 0};
-      if (valid) {
-        const int col = 16 * ks + 8 * (lane >> 5);
-        qf[ks] = *(const u32x4*)(a.q + b * a.q_sb + hq * a.q_sh + (int64_t)t * a.q_st + col);
-        df[ks] = *(const u32x4*)(dout + row + col);
-        float x[8], y[8], z[8];
-        up8<E>(df[ks], x);
-        up8<E>(*(const u32x4*)(o + row + col), y);
-        up8<E>(*(const u32x4*)(rest + row + col), z);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ds = fmaf(x[j], y[j] + z[j], ds);
-      }
-    }
-    ds = other_half(ds, false);
-    const float ls = lse[(int64_t)bh * nqb * BM + t];
     const uint16_t* kg = a.k + b * a.k_sb + hk * a.k_sh;
     const uint16_t* vg = a.v + b * a.v_sb + hk * a.v_sh;
     const Tiles tiles(s.st + bt0, s.st + bt1, a.W, a.S);
     auto fetch = [&](int it) {
-      fill_tile<D>(kg, a.k_st, tiles.key(it), 0, s.len, ring[it % NS][0], wave, lane);
-      fill_tile<D>(vg, a.v_st, tiles.key(it), 0, s.len, ring[it % NS][1], wave, lane);
+      fill_tile<D>(kg, a.k_st, tiles.key(it), 0, s.len, ring[(it + 1) % NS][0], wave, lane);
+      fill_tile<D>(vg, a.v_st, tiles.key(it), 0, s.len, ring[(it + 1) % NS][1], wave, lane);
     };
+    Rows<D>::fill(a.q + b * a.q_sb + hq * a.q_sh, a.q_st, tw, s.t0, s.t1, img, lane);
+    const float ls = lse[(int64_t)bh * nqb * BM + t];
+    // D of the wave's rows, from whole rows of do, o and its rest; do goes into the image behind q
+    const int64_t ld = (int64_t)a.H * D, base = ((int64_t)b * a.Tq * a.H + hq) * D;
+    u32x4 dr[Rows<D>::N];
+#pragma unroll
+    for (int j = 0; j < Rows<D>::N; ++j) {
+      const int r = j * PER + lane / CH;
+      const int64_t e = base + max(s.t0, min(s.t1 - 1, tw + r)) * ld + (lane % CH) * 8;
+      dr[j] = *(const u32x4*)(dout + e);
+      float x[8], y[8], z[8], part = 0.f;
+      up8<E>(dr[j], x);
+      up8<E>(*(const u32x4*)(o + e), y);
+      up8<E>(*(const u32x4*)(rest + e), z);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) part = fmaf(x[n], y[n] + z[n], part);
+#pragma unroll
+      for (int m = 1; m < CH; m <<= 1) part += __shfl_xor(part, m, 64);
+      if (lane % CH == 0) ds_s[wave * 32 + r] = part;
+    }
     for (int it = 0; it < min(NS - 1, tiles.n); ++it) fetch(it);
+    // (the q rows and everything before them: the loads of D above have waited for later ones)
+    u32x4 qf[DK], df[DK];
+    if (tiles.n >= NS - 1) wait_own<2 * kFills<D> * (NS - 1)>();
+    else wait_own<0>();
+    Rows<D>::read(img, qf, lane);
+#pragma unroll
+    for (int j = 0; j < Rows<D>::N; ++j)
+      *(u32x4*)(img + lds_off<D>(j * PER + lane / CH, (lane % CH) * 8)) = dr[j];
+    Rows<D>::read(img, df, lane);
+    ds = ds_s[wave * 32 + (lane & 31)];
     for (int it = 0; it < tiles.n; ++it) {
       if (it + NS - 1 <= tiles.n) wait_barrier<2 * kFills<D> * (NS - 2)>();
       else wait_barrier<0>();
       if (it + NS - 1 < tiles.n) fetch(it + NS - 1);
-      const uint16_t *Ks = ring[it % NS][0], *Vs = ring[it % NS][1];
+      const uint32_t Ks = lds_at(ring[(it + 1) % NS][0]), Vs = lds_at(ring[(it + 1) % NS][1]);
       if (wt0 > wt1) continue;
 #pragma unroll 1
       for (int sub = 0; sub < 2; ++sub) {
@@ -376,29 +441,35 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
         f32x16 x = zero16(), y = zero16();
 #pragma unroll
         for (int ks = 0; ks < DK; ++ks) {
-          x = E::mfma32(frag<D>(Ks, 32 * sub, ks, lane), qf[ks], x);
-          y = E::mfma32(frag<D>(Vs, 32 * sub, ks, lane), df[ks], y);
+          x = E::mfma32(at.frag(Ks + sub * 64 * D, 0, ks), qf[ks], x);
+          y = E::mfma32(at.frag(Vs + sub * 64 * D, 0, ks), df[ks], y);
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float p = __builtin_amdgcn_exp2f(fmaf(x[r], a.c, -ls));
-          if (see == 1) {
-            const int j = k0 + row_of(r, lane);
-            if (j > i || (i - j >= a.W && j >= a.S)) p = 0.f;
+        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.c, -ls)) * (y[r] - ds);
+        if (see == 1) {
+          const int d0 = i - k0 - 8 * (lane >> 5);
+          if (k0 >= a.S) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = (uint32_t)(d0 - row_of(r, 0)) < (uint32_t)a.W ? x[r] : 0.f;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              x[r] = (uint32_t)(d0 - row_of(r, 0)) < (k0 + row_of(r, lane) < a.S ? 1u << 31 : (uint32_t)a.W)
+                         ? x[r] : 0.f;
           }
-          x[r] = p * (y[r] - ds);
         }
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
           const u32x4 p = pack<E>(x, st);
 #pragma unroll
           for (int dn = 0; dn < DN; ++dn)
-            acc[dn] = E::mfma32(frag_t<D>(Ks, 32 * sub + 16 * st, dn, lane), p, acc[dn]);
+            acc[dn] = E::mfma32(at.frag_t(Ks + sub * 64 * D, 16 * st, dn), p, acc[dn]);
         }
       }
     }
   }
-  put_rows<E, D>(dq + ((int64_t)bh * a.Tq + t) * D, t < a.Tq, acc, valid ? scale : 0.f, lane);
+  __syncthreads();
+  Rows<D>::template put<E, false>(acc, valid ? scale : 0.f, dq + (int64_t)bh * a.Tq * D, D, tw, 0, a.Tq, img, lane);
   if (lane < 32) dsum[(int64_t)bh * nqb * BM + t] = valid ? ds : 0.f;
 }
 
@@ -411,10 +482,14 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
 // slot for each span); window_sink_kernel adds the slots.
 template <class E, int D>
 struct Dkv {
-  static constexpr int DK = D / 16, DN = D / 32, NS = kRing<D>;
+  // heads of 128: 64 registers of key and value fragments beside 128 of sums leave too few for the
+  // rest; the values stay in LDS, and tiles of 32 queries make room for them
+  static constexpr bool kValuesInLds = D == 128;
+  static constexpr int DK = D / 16, DN = D / 32, NS = kBwdRing<D>, QN = D == 128 ? 32 : BN, SUBS = QN / 32;
   struct Lds {
-    uint16_t ring[NS][2][BN * D];
-    float stat[NS][2][BN];                             // log-sums, D
+    uint16_t ring[NS][2][QN * D];
+    uint16_t values[kValuesInLds ? BM * D : 8];
+    float stat[NS][2][64];                             // log-sums, D
   };
   static constexpr float kUnshift = 1.f / (1 << E::kShift);   // (elt.h: p is 2^kShift times its value)
   const WinArgs& a;
@@ -423,96 +498,126 @@ struct Dkv {
   Lds& lds;
   const Seq& s;
   int b, hk, tq_pad, tid, lane, wave;
-  u32x4 kf[DK], vf[DK];
+  Place<D> at;
+  u32x4 kf[DK], vf[kValuesInLds ? 1 : DK];
   f32x16 ak[DN], av[DN];
 
-  // keys kw ... kw + 31 as B operands (zeros behind the sequence), accumulators cleared
-  __device__ __forceinline__ void begin(int kw) {
-    const int j = kw + (lane & 31);
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int dn = 0; dn < DN; ++dn) ak[dn] = av[dn] = zero16();
-#pragma unroll
-    for (int ks = 0; ks < DK; ++ks) {
-      kf[ks] = vf[ks] = u32x4{0, 0, 0, 0};
-      if (j < s.len) {
-        const int col = 16 * ks + 8 * (lane >> 5);
-        kf[ks] = *(const u32x4*)(a.k + b * a.k_sb + hk * a.k_sh + (int64_t)j * a.k_st + col);
-        vf[ks] = *(const u32x4*)(a.v + b * a.v_sb + hk * a.v_sh + (int64_t)j * a.v_st + col);
-      }
-    }
   }
 
   // query tile it of `per` tiles a head, the first at row tb
   __device__ __forceinline__ void fetch(int it, int per, int tb) {
-    const int G = a.H / a.KV, hq = hk * G + it / per, row0 = tb + (it % per) * BN, slot = it % NS;
-    fill_tile<D>(a.q + b * a.q_sb + hq * a.q_sh, a.q_st, row0, s.t0, s.t1, lds.ring[slot][0], wave, lane);
-    fill_tile<D>(dout + ((int64_t)b * a.Tq * a.H + hq) * D, (int64_t)a.H * D, row0, s.t0, s.t1,
-                 lds.ring[slot][1], wave, lane);
+    const int G = a.H / a.KV, hq = hk * G + it / per, row0 = tb + (it % per) * QN, slot = (it + 2) % NS;
+    fill_tile<D, QN>(a.q + b * a.q_sb + hq * a.q_sh, a.q_st, row0, s.t0, s.t1, lds.ring[slot][0], wave, lane);
+    fill_tile<D, QN>(dout + ((int64_t)b * a.Tq * a.H + hq) * D, (int64_t)a.H * D, row0, s.t0, s.t1,
+                     lds.ring[slot][1], wave, lane);
     // (waves 2 and 3 write what waves 0 and 1 do: each has the same number of loads under way)
-    fill4(((wave & 1) ? dsum : lse) + ((int64_t)b * a.H + hq) * tq_pad + row0 + lane, lds.stat[slot][wave & 1]);
+    fill4(scalar(((wave & 1) ? dsum : lse) + ((int64_t)b * a.H + hq) * tq_pad + row0),
+          4 * (lane & (QN - 1)), lds.stat[slot][wave & 1]);
   }
 
-  // queries 32 sub ... of the tile against this wave's keys; ALL: every pair counts
-  template <bool FAR>
-  __device__ __forceinline__ void step(int slot, int sub, int p0, int kw, bool all) {
-    const uint16_t *Qs = lds.ring[slot][0], *Os = lds.ring[slot][1];
+  // All tiles of rows [t0, t1) of every query head, for the pairs with lo <= i - j < lo + n: the
+  // window's (0, W), or far ones (W, as many as there may be; j < S)
+  __device__ __forceinline__ void run(bool far, int kw, int t0, int t1) {
+    const int tb = t0 & ~(QN - 1), per = (t1 - 1 - tb) / QN + 1, tiles = per * (a.H / a.KV);
+    constexpr int kTile = 2 * kFills<D, QN> + 1;
+    // the wave's keys and values: slots 0 and 1 of three; heads of 128: both slots, and the values' place
+    uint16_t* img = lds.ring[0][0] + wave * Rows<D>::SIZE;
+    uint16_t* vimg = kValuesInLds ? lds.values + wave * Rows<D>::SIZE : img + 4 * Rows<D>::SIZE;
+    Rows<D>::fill(a.k + b * a.k_sb + hk * a.k_sh, a.k_st, kw, 0, s.len, img, lane);
+    Rows<D>::fill(a.v + b * a.v_sb + hk * a.v_sh, a.v_st, kw, 0, s.len, vimg, lane);
+    int issued = 0;
+    if (NS == 3) {                                     // (a tile goes into the third slot)
+      fetch(issued++, per, tb);
+      wait_own<kTile>();
+    } else {
+      wait_own<0>();
+    }
+    Rows<D>::read(img, kf, lane);
+    if constexpr (!kValuesInLds) Rows<D>::read(vimg, vf, lane);
+    if (NS == 2) {
+      wait_barrier<0>();
+      fetch(issued++, per, tb);
+    }
+    const int j = kw + (lane & 31), lo = far ? a.W : 0;
+    const uint32_t n = far ? 1u << 30 : (uint32_t)a.W, mine = far && j >= a.S ? 0 : n;
+    for (int it = 0; it < tiles; ++it) {
+      if (issued - it - 1 == NS - 2) wait_barrier<kTile * (NS - 2)>();
+      else wait_barrier<0>();
+      while (issued < min(tiles, it + NS)) fetch(issued++, per, tb);
+      const int row0 = tb + (it % per) * QN;
+#pragma unroll 1
+      for (int sub = 0; sub < SUBS; ++sub) {
+        if (far && ((it * SUBS + sub) & 3) != wave) continue;
+        const int least = s.st + row0 + 32 * sub - kw - 31;   // of i - j; the largest is 62 more
+        if (least + 62 < lo || (least >= lo && (uint32_t)(least - lo) >= n)) continue;
+        const bool all = least >= lo && (uint32_t)(least + 62 - lo) < n && (!far || kw + 31 < a.S);
+        step((it + 2) % NS, sub, all, least + 31 + kw - j - lo, mine);
+      }
+    }
+  }
+
+  // queries 32 sub ... of the tile against this wave's keys.  d0: i - j - lo of the first query and
+  // this lane's key, pairs with values of [0, mine) count (all: every pair does)
+  __device__ __forceinline__ void step(int slot, int sub, bool all, int d0, uint32_t mine) {
+    const uint32_t Qs = lds_at(lds.ring[slot][0]) + sub * 64 * D, Os = lds_at(lds.ring[slot][1]) + sub * 64 * D;
     const float *ls = lds.stat[slot][0], *ds = lds.stat[slot][1];
     f32x16 x = zero16(), y = zero16();
 #pragma unroll
-    for (int ks = 0; ks < DK; ++ks) {
-      x = E::mfma32(frag<D>(Qs, 32 * sub, ks, lane), kf[ks], x);
-      y = E::mfma32(frag<D>(Os, 32 * sub, ks, lane), vf[ks], y);
-    }
-    const int j = kw + (lane & 31);
+    for (int ks = 0; ks < DK; ++ks) x = E::mfma32(at.frag(Qs, 0, ks), kf[ks], x);
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
-      const int q0 = row_of(4 * r4, lane);
-      const f32x4 l4 = *(const f32x4*)(ls + 32 * sub + q0), d4 = *(const f32x4*)(ds + 32 * sub + q0);
+      const f32x4 l4 = *(const f32x4*)(ls + 32 * sub + row_of(4 * r4, lane));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * r4 + e;
-        float p = __builtin_amdgcn_exp2f(fmaf(x[r], a.c, (float)E::kShift - l4[e]));
-        if (!all) {
-          const int d = p0 + q0 + e - j;               // i - j
-          if (FAR ? (j >= a.S || d < a.W) : (d < 0 || d >= a.W)) p = 0.f;
-        }
-        x[r] = p;
-        y[r] = p * fmaf(d4[e], -kUnshift, y[r] * kUnshift);
+      for (int e = 0; e < 4; ++e)
+        x[4 * r4 + e] = __builtin_amdgcn_exp2f(fmaf(x[4 * r4 + e], a.c, (float)E::kShift - l4[e]));
+    }
+    if (!all) {
+      const int d = d0 + 8 * (lane >> 5);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = (uint32_t)(d + row_of(r, 0)) < mine ? x[r] : 0.f;
+    }
+    if (D == 128) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ks = 0; ks < DK; ++ks) {
+      u32x4 f;
+      if constexpr (kValuesInLds)
+        f = lds16(lds.values + wave * Rows<D>::SIZE + lds_off<D>(lane & 31, 16 * ks + 8 * (lane >> 5)));
+      else
+        f = vf[ks];
+      y = E::mfma32(at.frag(Os, 0, ks), f, y);
+    }
+    if constexpr (D == 128) {                          // reads two products ahead, not all at once
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int ks = 0; ks < DK - 2; ++ks) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       }
+      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const f32x4 d4 = *(const f32x4*)(ds + 32 * sub + row_of(4 * r4, lane));
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y[4 * r4 + e] = x[4 * r4 + e] * (E::kShift ? fmaf(d4[e], -kUnshift, y[4 * r4 + e] * kUnshift)
+                                                   : y[4 * r4 + e] - d4[e]);
     }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
-      const u32x4 p = pack<E>(x, st), d = pack<E>(y, st);
+      const u32x4 p = pack<E>(x, st);
 #pragma unroll
-      for (int dn = 0; dn < DN; ++dn) {
-        av[dn] = E::mfma32(frag_t<D>(Os, 32 * sub + 16 * st, dn, lane), p, av[dn]);
-        ak[dn] = E::mfma32(frag_t<D>(Qs, 32 * sub + 16 * st, dn, lane), d, ak[dn]);
-      }
+      for (int dn = 0; dn < DN; ++dn) av[dn] = E::mfma32(at.frag_t(Os, 16 * st, dn), p, av[dn]);
     }
-  }
-
-  // all tiles of rows [t0, t1) of every query head
-  template <bool FAR>
-  __device__ __forceinline__ void run(int kw, int t0, int t1) {
-    const int tb = t0 & ~(BN - 1), per = (t1 - 1 - tb) / BN + 1, n = per * (a.H / a.KV);
-    for (int it = 0; it < min(NS - 1, n); ++it) fetch(it, per, tb);
-    for (int it = 0; it < n; ++it) {
-      if (it + NS - 1 <= n) wait_barrier<(2 * kFills<D> + 1) * (NS - 2)>();
-      else wait_barrier<0>();
-      if (it + NS - 1 < n) fetch(it + NS - 1, per, tb);
-      const int row0 = tb + (it % per) * BN;
-      if (FAR) {
-        if ((it & 1) != (wave >> 1)) continue;
-        const int sub = wave & 1, p0 = s.st + row0 + 32 * sub;
-        if (p0 + 31 - kw >= a.W) step<true>(it % NS, sub, p0, kw, kw + 31 < a.S && p0 - (kw + 31) >= a.W);
-      } else {
-#pragma unroll 1
-        for (int sub = 0; sub < 2; ++sub) {
-          const int p0 = s.st + row0 + 32 * sub;
-          if (p0 + 31 < kw || p0 - (kw + 31) >= a.W) continue;
-          step<false>(it % NS, sub, p0, kw, p0 >= kw + 31 && p0 + 31 - kw < a.W);
-        }
-      }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const u32x4 d = pack<E>(y, st);
+#pragma unroll
+      for (int dn = 0; dn < DN; ++dn) ak[dn] = E::mfma32(at.frag_t(Qs, 16 * st, dn), d, ak[dn]);
     }
   }
 
@@ -552,35 +657,39 @@ __global__ __launch_bounds__(256, kDkvWaves<D>) void window_dkv_kernel(WinArgs a
                                                          float* part, int spans, int span, float scale) {
   using K = Dkv<E, D>;
   static_assert(sizeof(typename K::Lds) >= 3 * 64 * D / 2 * 4, "room to join the waves");
-  __shared__ __attribute__((aligned(16))) typename K::Lds lds;
+  __shared__ __attribute__((aligned(256))) typename K::Lds lds;
   const int nkb = (a.Tk + BM - 1) / BM;
   const int nst = spans ? (a.S + 31) / 32 : 0, items = nkb + nst * spans;
   const int item = xcd_remap((int)blockIdx.x, (int)gridDim.x);
   const int bk = item / items, it0 = item - bk * items, b = bk / a.KV, hk = bk - b * a.KV;
   const Seq s = seq_of(a, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  K k{a, dout, lse, dsum, lds, s, b, hk, (a.Tq + BM - 1) / BM * BM, tid, lane, wave};
-  if (it0 < nst * spans) {
-    const int c = it0 % spans, kw = it0 / spans * 32, j = kw + (lane & 31);
-    const int t0 = (int)max((int64_t)max(s.t0, c * span), (int64_t)a.W + kw - s.st);
-    const int t1 = (int)min((int64_t)s.t1, (int64_t)(c + 1) * span);
-    k.begin(kw);
-    if (t0 < t1 && kw < s.len) k.template run<true>(kw, t0, t1);
+  K k{a, dout, lse, dsum, lds, s, b, hk, (a.Tq + BM - 1) / BM * BM, tid, lane, wave, Place<D>(lane)};
+  const bool far = it0 < nst * spans;
+  const int c = far ? it0 % spans : 0;
+  const int kb = it0 - nst * spans, kw = far ? it0 / spans * 32 : kb * BM + wave * 32, j = kw + (lane & 31);
+  // near: queries of positions [kb BM, last key + W)
+  int t0 = max(s.t0, kb * BM - s.st);
+  int t1 = (int)min((int64_t)s.t1, (int64_t)kb * BM + BM - 1 + a.W - s.st);
+  if (far) {
+    t0 = max(max(s.t0, c * span), a.W + kw - s.st);
+    t1 = (int)min((int64_t)s.t1, (int64_t)(c + 1) * span);
+  }
+  k.clear();
+  if (t0 < t1 && (far ? kw : kb * BM) < s.len) k.run(far, kw, t0, t1);
+  if (far) {
     k.join(k.ak);
     k.join(k.av);
     if (!wave && j < a.S) k.put_part(part + (((int64_t)(1 + c) * a.B * a.KV + bk) * a.S + j) * 2 * D);
     return;
   }
-  const int kb = it0 - nst * spans, kw = kb * BM + wave * 32, j = kw + (lane & 31);
-  // positions [kb BM, last key + W)
-  const int t0 = max(s.t0, kb * BM - s.st);
-  const int t1 = (int)min((int64_t)s.t1, (int64_t)kb * BM + BM - 1 + a.W - s.st);
-  k.begin(kw);
-  if (t0 < t1 && kb * BM < s.len) k.template run<false>(kw, t0, t1);
   const bool sink = spans && j < a.S;
-  const int64_t row = ((int64_t)bk * a.Tk + j) * D;
-  put_rows<E, D>(dk + row, j < a.Tk && !sink, k.ak, scale, lane);
-  put_rows<E, D>(dv + row, j < a.Tk && !sink, k.av, K::kUnshift, lane);
+  uint16_t* img = lds.ring[0][0] + wave * Rows<D>::SIZE;
+  const int64_t base = (int64_t)bk * a.Tk * D;
+  const int lo = spans ? a.S : 0;                      // (rows of sinks: window_sink_kernel)
+  __syncthreads();
+  Rows<D>::template put<E, false>(k.ak, scale, dk + base, D, kw, lo, a.Tk, img, lane);
+  Rows<D>::template put<E, false>(k.av, K::kUnshift, dv + base, D, kw, lo, a.Tk, img, lane);
   if (sink) k.put_part(part + ((int64_t)bk * a.S + j) * 2 * D);
 }
 
@@ -601,6 +710,212 @@ __global__ __launch_bounds__(256) void window_sink_kernel(const float* part, int
   v *= which ? 1.f / (1 << E::kShift) : scale;
   *(uint2*)((which ? dv : dk) + ((int64_t)bk * Tk + j) * D + c) =
       make_uint2(E::pack2(v[0], v[1]), E::pack2(v[2], v[3]));
+}
+
+// ------------------------------------------------------------------------------------ few queries
+// Forward for at most 16 rows of (query head of one key head, token): one token of a cache, mostly.
+// What counts there is that the keys and values are read once at full rate, so a workgroup is 8 waves
+// that go through the keys 32 at a time on their own -- keys from memory into registers as operands,
+// values into LDS for the transposing read, both a chunk ahead -- and join their maxima, sums and
+// products in the end.  With `splits` > 1 the keys of a head are shared among that many workgroups,
+// which leave theirs in `part`, and window_join_kernel joins them.
+// Products are 16x16x32: lane l holds A[l & 15][8 (l >> 4) ..], B[8 (l >> 4) ..][l & 15] and
+// C[4 (l >> 4) + r][l & 15]; the keys of the two score tiles of a chunk are fed so that a lane's
+// 4 + 4 scores are those of keys 8 (l >> 4) ... + 7, the B operand of the product with V.
+constexpr int NW = 8;          // (64 sequences of 4 key heads of 64, 1028 keys: 13.8 us, with 16 waves 15.3)
+
+__device__ __forceinline__ float over_groups(float v, bool mx) {      // lanes l, l ^ 16, l ^ 32, l ^ 48
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  const float a = __uint_as_float(p[0]), b = __uint_as_float(p[1]);
+  return other_half(mx ? fmaxf(a, b) : a + b, mx);
+}
+
+template <class E, int D>
+__global__ __launch_bounds__(NW * 64) void window_step_kernel(WinArgs a, uint16_t* o, float* part, int splits) {
+  constexpr int DK = D / 32, DT = D / 16;
+  __shared__ __attribute__((aligned(256))) uint16_t vs[NW][2][32 * D];
+  __shared__ float stat[2][NW][16];
+  const int G = a.H / a.KV, rows = G * a.Tq;
+  const int bk = blockIdx.x / splits, split = blockIdx.x - bk * splits, b = bk / a.KV, hk = bk - b * a.KV;
+  const Seq s = seq_of(a, b);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int li = lane & 15, g = lane >> 4;
+  const int t = li % a.Tq, hq = hk * G + li / a.Tq;            // this lane's row
+  const bool valid = li < rows && t >= s.t0 && t < s.t1;
+  const int i = valid ? s.st + t : -1;
+
+  f32x4 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0, 0, 0, 0};
+  float m = -3e38f, l = 0.f;
+  if (s.t0 < s.t1) {
+    const uint16_t* kg = a.k + b * a.k_sb + hk * a.k_sh;
+    const uint16_t* vg = a.v + b * a.v_sb + hk * a.v_sh;
+    u32x4 qf[DK];
+#pragma unroll
+    for (int ks = 0; ks < DK; ++ks) {
+      qf[ks] = u32x4{0, 0, 0, 0};
+      if (valid) qf[ks] = *(const u32x4*)(a.q + b * a.q_sb + hq * a.q_sh + (int64_t)t * a.q_st + 32 * ks + 8 * g);
+    }
+    // chunks of 32 keys: sinks in front of the window, then the window; this workgroup's share
+    const int low = max(0, s.st + s.t0 - a.W + 1) & ~31, last = s.st + s.t1 - 1;
+    const int sinks = (min(a.S, low) + 31) / 32, n = sinks + (last - low) / 32 + 1;
+    const int per = (n + splits - 1) / splits, end = min(n, (split + 1) * per);
+    auto key = [&](int c) { return 32 * (c < sinks ? c : c - sinks) + (c < sinks ? 0 : low); };
+    u32x4 kf[2][DK];
+    auto fetch = [&](int c, int buf) {
+      const int k0 = key(c);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // (what the buffer held has been read)
+      Rows<D>::fill(vg, a.v_st, k0, 0, s.len, vs[wave][buf], lane);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t row = (int64_t)min(s.len - 1, k0 + 8 * (li >> 2) + 4 * h + (li & 3)) * a.k_st;
+#pragma unroll
+        for (int ks = 0; ks < DK; ++ks) kf[h][ks] = *(const u32x4*)(kg + row + 32 * ks + 8 * g);
+      }
+    };
+    int c = split * per + wave, buf = 0;
+    if (c < end) fetch(c, 0);
+    for (; c < end; c += NW, buf ^= 1) {
+      const int k0 = key(c);
+      f32x4 x[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        x[h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < DK; ++ks) x[h] = E::mfma16(kf[h][ks], qf[ks], x[h]);
+      }
+      // (the keys, loaded behind them, are here: so are the values)
+      if (c + NW < end) fetch(c + NW, buf ^ 1);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = k0 + 8 * g + 4 * h + r;
+          const bool see = j <= i && (i - j < a.W || j < a.S);
+          x[h][r] = see ? x[h][r] * a.c : -INFINITY;
+          mx = fmaxf(mx, x[h][r]);
+        }
+      const float mn = fmaxf(m, over_groups(mx, true)), f = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[h][r] = __builtin_amdgcn_exp2f(x[h][r] - m);
+          sum += x[h][r];
+        }
+      l = l * f + sum;
+      const u32x4 p = {E::pack2(x[0][0], x[0][1]), E::pack2(x[0][2], x[0][3]), E::pack2(x[1][0], x[1][1]),
+                       E::pack2(x[1][2], x[1][3])};
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const uint16_t* v = vs[wave][buf];
+        const int r = 8 * g + (li >> 2), col = 16 * dt + 4 * (li & 3);
+        const bf16x8 vf = cat_frag(lds_tr4((const bf16_t*)v + lds_off<D>(r, col)),
+                                   lds_tr4((const bf16_t*)v + lds_off<D>(r + 4, col)));
+        acc[dt] *= f;
+        acc[dt] = E::mfma16(__builtin_bit_cast(u32x4, vf), p, acc[dt]);
+      }
+    }
+    l = over_groups(l, false);
+  }
+  // the waves' rows are joined relative to the largest of their maxima
+  if (lane < 16) {
+    stat[0][wave][lane] = m;
+    stat[1][wave][lane] = l;
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+  float* buf = (float*)vs;                             // [NW][16][D]
+  float top = -3e38f, total = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) top = fmaxf(top, stat[0][w][li]);
+#pragma unroll
+  for (int w = 0; w < NW; ++w) total += stat[1][w][li] * __builtin_amdgcn_exp2f(stat[0][w][li] - top);
+  const float f = __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) *(f32x4*)(buf + (wave * 16 + li) * D + 16 * dt + 4 * g) = acc[dt] * f;
+  __syncthreads();
+  // thread: row e / (D / 4), 4 columns
+  for (int e = tid; e < rows * (D / 4); e += NW * 64) {
+    const int row = e / (D / 4), col = e % (D / 4) * 4;
+    f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += *(const f32x4*)(buf + (w * 16 + row) * D + col);
+    if (splits > 1) {
+      *(f32x4*)(part + ((int64_t)blockIdx.x * 16 + row) * (D + 4) + col) = v;
+    } else {
+      float tm = -3e38f, z = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) tm = fmaxf(tm, stat[0][w][row]);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) z += stat[1][w][row] * __builtin_amdgcn_exp2f(stat[0][w][row] - tm);
+      v *= z > 0.f ? 1.f / z : 0.f;
+      const int64_t at = (((int64_t)b * a.Tq + row % a.Tq) * a.H + hk * G + row / a.Tq) * D + col;
+      *(uint2*)(o + at) = make_uint2(E::pack2(v[0], v[1]), E::pack2(v[2], v[3]));
+    }
+  }
+  if (splits > 1 && wave == 0 && lane < rows) {
+    float* st = part + ((int64_t)blockIdx.x * 16 + lane) * (D + 4) + D;
+    st[0] = top;
+    st[1] = total;
+  }
+}
+
+// one row of a key head from the shares of its workgroups: thread (slice, 4 columns)
+template <class E, int D>
+__global__ __launch_bounds__(256) void window_join_kernel(const float* part, int splits, uint16_t* o, int H, int KV,
+                                                          int Tq) {
+  constexpr int C = D / 4, SL = 256 / C;
+  constexpr int64_t step = 16 * (D + 4);
+  __shared__ float tops[4];
+  __shared__ f32x4 sums[SL][C];
+  __shared__ float zs[SL];
+  const int G = H / KV, rows = G * Tq, bk = blockIdx.x / rows, row = blockIdx.x - bk * rows;
+  const int b = bk / KV, hk = bk - b * KV, tid = threadIdx.x;
+  const float* p = part + ((int64_t)bk * splits * 16 + row) * (D + 4);
+  float top = -3e38f;
+  for (int i = tid; i < splits; i += 256) top = fmaxf(top, p[i * step + D]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const int sl = tid / C, col = tid % C * 4;
+  float z = 0.f;
+  f32x4 v = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int i = sl; i < splits; i += SL) {
+    const float f = __builtin_amdgcn_exp2f(p[i * step + D] - top);
+    z += p[i * step + D + 1] * f;
+    v += *(const f32x4*)(p + i * step + col) * f;
+  }
+  sums[sl][col / 4] = v;
+  if (col == 0) zs[sl] = z;
+  __syncthreads();
+  if (sl) return;
+  for (int i = 1; i < SL; ++i) {
+    v += sums[i][col / 4];
+    z += zs[i];
+  }
+  v *= z > 0.f ? 1.f / z : 0.f;
+  const int64_t at = (((int64_t)b * Tq + row % Tq) * H + hk * G + row / Tq) * D + col;
+  *(uint2*)(o + at) = make_uint2(E::pack2(v[0], v[1]), E::pack2(v[2], v[3]));
+}
+
+template <class E, int D>
+int step(const WinArgs& a, void* o, void* part, int splits, hipStream_t st) {
+  const int64_t n = (int64_t)a.B * a.KV * splits;
+  if (n >= (1ll << 31) || (int64_t)a.B * a.H * a.Tq >= (1ll << 31)) return 1;
+  hipLaunchKernelGGL((window_step_kernel<E, D>), dim3((unsigned)n), dim3(NW * 64), 0, st, a, (uint16_t*)o,
+                     (float*)part, splits);
+  if (splits > 1)
+    hipLaunchKernelGGL((window_join_kernel<E, D>), dim3((unsigned)((int64_t)a.B * a.H * a.Tq)), dim3(256), 0, st, (const float*)part, splits,
+                       (uint16_t*)o, a.H, a.KV, a.Tq);
+  return (int)hipGetLastError();
 }
 
 template <class E, int D>
@@ -637,7 +952,7 @@ int bwd(const WinArgs& a, const void* o, const void* rest, const void* dout, con
 bool good(const WinArgs& a, int D) {
   return a.B > 0 && a.H > 0 && a.KV > 0 && a.H % a.KV == 0 && a.Tq > 0 && a.Tk > 0 && a.W > 0 && a.S >= 0 &&
          (D == 64 || D == 128) && a.Tq <= (1 << 29) && a.Tk <= (1 << 29) && a.W <= (1 << 30) &&
-         a.S <= a.Tk && a.c > 0.f;
+         a.S <= a.Tk && (int64_t)a.H * D < (1 << 24) && a.c > 0.f;
 }
 
 WinArgs args(const void* q, const void* k, const void* v, const int64_t* s, const void* start, const void* lengths,
@@ -662,6 +977,17 @@ int mopt_window_fwd(const void* q, const void* k, const void* v, const int64_t* 
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) return D == 64 ? fwd<Bf16, 64>(a, o, rest, lse, st) : fwd<Bf16, 128>(a, o, rest, lse, st);
   return D == 64 ? fwd<Fp16, 64>(a, o, rest, lse, st) : fwd<Fp16, 128>(a, o, rest, lse, st);
+}
+
+// The same output for H / KV * Tq <= 16; part: workspace of B KV splits 16 (D + 4) floats where splits > 1.
+int mopt_window_step(const void* q, const void* k, const void* v, const int64_t* strides, const void* start,
+                     const void* lengths, int start0, void* o, void* part, int splits, int B, int H, int KV, int Tq,
+                     int Tk, int D, int W, int S, float scale, int dtype, void* stream) {
+  const WinArgs a = args(q, k, v, strides, start, lengths, start0, B, H, KV, Tq, Tk, W, S, scale);
+  if (!good(a, D) || (int64_t)(H / KV) * Tq > 16 || splits < 1 || (splits > 1 && !part)) return 1;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == 0) return D == 64 ? step<Bf16, 64>(a, o, part, splits, st) : step<Bf16, 128>(a, o, part, splits, st);
+  return D == 64 ? step<Fp16, 64>(a, o, part, splits, st) : step<Fp16, 128>(a, o, part, splits, st);
 }
 
 // dq [B][H][Tq][D], dk, dv [B][KV][Tk][D]; dsum: floats of workspace; part: workspace of

@@ -29,6 +29,8 @@ _lib.register_signatures({
                               [c_float, c_int, c_int, c_void_p], c_int),
     "mopt_window_fwd": ([c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int] * 8 +
                         [c_float, c_int, c_void_p], c_int),
+    "mopt_window_step": ([c_void_p] * 6 + [c_int] + [c_void_p] * 2 + [c_int] * 9 +
+                         [c_float, c_int, c_void_p], c_int),
     "mopt_window_bwd": ([c_void_p] * 6 + [c_int] + [c_void_p] * 9 + [c_int] * 10 +
                         [c_float, c_int, c_void_p], c_int),
 })
@@ -55,7 +57,8 @@ def _p(t: Optional[torch.Tensor]):
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """``t`` with contiguous 16-byte aligned rows (a copy only where it has none)."""
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]):
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]) or \
+            t.stride(-2) >= 1 << 24:           # (a tile's 64 rows are reached by 32-bit offsets)
         return t.contiguous() if not t.is_contiguous() else t.clone()
     return t
 
@@ -293,6 +296,13 @@ def _geometry(q, k, v):
     return (c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
 
 
+def _splits(heads: int, tokens: int) -> int:
+    """Workgroups that share the ``tokens`` keys of each of ``heads`` key heads: at most one a CU
+    over all heads (32768 keys of 8 heads: 26 us, with two a CU 30), and each with 1024 keys at
+    least: joining them costs a launch, 3.4 us, as much as about 1000 keys do."""
+    return max(1, min(256 // heads, tokens // 1024))
+
+
 def _window_fwd(q, k, v, window, sinks, scale, start, start0, lengths, train):
     B, H, Tq, D = q.shape
     KV, Tk = k.shape[1], k.shape[2]
@@ -300,7 +310,14 @@ def _window_fwd(q, k, v, window, sinks, scale, start, start0, lengths, train):
     # for the backward: the log-sums and what the rounding of o left off
     lse = torch.empty(B, H, -(-Tq // 128) * 128, dtype=torch.float32, device=q.device) if train else None
     rest = torch.empty_like(o) if train else None
-    if o.numel() and Tk:
+    if o.numel() and Tk and not train and H // KV * Tq <= 16:
+        splits = _splits(B * KV, min(Tk, window + sinks))
+        part = torch.empty(B * KV * splits * 16 * (D + 4), dtype=torch.float32,
+                           device=q.device) if splits > 1 else None
+        _call(q, "mopt_window_step", _p(q), _p(k), _p(v), _geometry(q, k, v), _p(start), _p(lengths),
+              start0, _p(o), _p(part), splits, B, H, KV, Tq, Tk, D, window, sinks, scale,
+              _TYPES[q.dtype])
+    elif o.numel() and Tk:
         _call(q, "mopt_window_fwd", _p(q), _p(k), _p(v), _geometry(q, k, v), _p(start), _p(lengths),
               start0, _p(o), _p(rest), _p(lse), B, H, KV, Tq, Tk, D, window, sinks, scale,
               _TYPES[q.dtype])
