@@ -7,9 +7,12 @@
 //   dx_j = (1 - a) (p1_j - [j = y]) + a tau (ptau_j - sum_k q_k [i_k = j])
 // A row without a label has no first term, one without a teacher no second.
 //
-// One workgroup per row.  The row is read once, into registers (lm_distill_row with NCH 16-byte
-// chunks a thread): its maximum, then both sums of exponentials, then the gradient come from
-// there, so the traffic is one read and one write of the logits.  The K + 1 corrected places of
+// One workgroup per row.  The row is read once, into registers (distill_row_kernel with NCH 16-byte
+// chunks a thread): its maximum, then both sums of exponentials, then the gradient come from there,
+// so the traffic is one read and one write of the logits, which bounds it (32768 rows of 32000 bf16
+// logits, K = 64: 850 us a pass, 4.9 TB/s, as fast as a copy of 4 GiB; before the row's floats were
+// kept from being held unpacked, at half the occupancy, 951).  Two exponentials a value in each of
+// the two passes hide behind it: at temperature 1, where one would do, the time is the same.  The K + 1 corrected places of
 // the gradient are written again after the dense pass with their whole f32 value, so each value
 // is rounded once; equal indices are added up by every entry that has them.  Sums of losses are
 // taken row by row in a fixed order (no atomics).
@@ -111,13 +114,13 @@ __device__ __forceinline__ float load_top(const void* p, int type, int64_t i) {
 }
 
 // The compiler would keep the unpacked floats of the row from one pass to the next, in twice the
-// registers: a value that went through this is unpacked anew.
-__device__ __forceinline__ void forget(u32x4& v) { asm("" : "+v"(v)); }
+// registers: a value that went through this is unpacked anew, chunk after chunk (volatile: in order).
+__device__ __forceinline__ void forget(u32x4& v) { asm volatile("" : "+v"(v)); }
 
 // NCH > 0: the row is kept in NCH chunks of NT threads (V <= NT * NCH * N).  NCH = 0: longer rows
-// are read again from memory in each pass.
-template <class E, int NT, int NCH>
-__global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
+// are read again from memory in each pass.  WAVES a SIMD: the registers (512 / WAVES).
+template <class E, int NT, int NCH, int WAVES>
+__global__ __launch_bounds__(NT, WAVES) void distill_row_kernel(DistillArgs a) {
   using R = Row<E>;
   using C = typename Chunk<R::SIZE>::type;
   constexpr int N = R::N;
@@ -128,36 +131,44 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
   const int tid = threadIdx.x, V = a.V, K = a.K;
   const int64_t row = blockIdx.x;
   const int trial = (int)(row / a.rpt);
-  const char* x = (const char*)a.x + row * a.ld * R::SIZE;
+  const char* const x = (const char*)a.x + row * a.ld * R::SIZE;
   const float tau = a.tau ? a.tau[trial] : a.tau_v, alpha = a.alpha ? a.alpha[trial] : a.alpha_v;
   const float rtau = 1.f / tau;
-  const int chunks = (V + N - 1) / N;
 
-  auto fetch = [&](int c, float (&f)[N]) {          // chunk c of the row, -inf behind its end
-    if ((c + 1) * N <= V) {
-      R::get(((const C*)x)[c].v, f);
-    } else {
+  // whole chunks, and the few values behind them: one more of the first threads
+  const int full = V / N;
+  const float more = tid < V - full * N ? R::load(x, full * N + tid) : -INFINITY;
+  float none[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) f[j] = c * N + j < V ? R::load(x, c * N + j) : -INFINITY;
-    }
-  };
+  for (int j = 0; j < N; ++j) none[j] = -INFINITY;
   u32x4 keep[NCH > 0 ? NCH : 1];
-  float mx[2] = {-INFINITY, -INFINITY};             // of the row, of the teacher
   if constexpr (NCH > 0) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = i * NT + tid;
-      if ((c + 1) * N <= V) {
-        keep[i] = ((const C*)x)[c].v;
-      } else {
-        float f[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = c * N + j < V ? R::load(x, c * N + j) : -INFINITY;
-        keep[i] = R::put(f);
-      }
+      keep[i] = R::put(none);
+      if (i * NT + tid < full) keep[i] = ((const C*)(x + i * NT * 16))[tid].v;   // (scalar base, one offset)
     }
   }
-  int y = a.labels[row];
+  // every chunk of this thread, in its order: f(first chunk of the group, values)
+  auto each = [&](auto f) {
+    if constexpr (NCH > 0) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        float v[N];
+        forget(keep[i]);
+        R::get(keep[i], v);
+        f(i * NT, v);
+      }
+    } else {
+      for (int c = 0; c + tid < full; c += NT) {
+        float v[N];
+        R::get(((const C*)(x + c * 16))[tid].v, v);
+        f(c, v);
+      }
+    }
+  };
+  float mx[2] = {more, -INFINITY};                  // of the row, of the teacher
+  const int y = a.labels[row];
   const bool has_label = y >= 0 && y < V;
   const float xy = has_label ? R::load(x, y) : 0.f;
   for (int k = tid; k < K; k += NT) {
@@ -168,53 +179,34 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
     s_e[k] = t;                                      // (each thread reads back its own entries)
     mx[1] = fmaxf(mx[1], t);
   }
-  if constexpr (NCH > 0) {
+  each([&](int, const float (&f)[N]) {
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      float f[N];
-      R::get(keep[i], f);
-#pragma unroll
-      for (int j = 0; j < N; ++j) mx[0] = fmaxf(mx[0], f[j]);
-    }
-  } else {
-    for (int c = tid; c < chunks; c += NT) {
-      float f[N];
-      fetch(c, f);
-#pragma unroll
-      for (int j = 0; j < N; ++j) mx[0] = fmaxf(mx[0], f[j]);
-    }
-  }
+    for (int j = 0; j < N; ++j) mx[0] = fmaxf(mx[0], f[j]);
+  });
   block_all<NT, 2, true>(mx, red);
   const float m = mx[0], tm = mx[1];
-  const float k1 = kLog2e, kt = kLog2e * rtau;
+  // (the reference is in the exponent's fma: what its rounding changes is a factor of all terms)
+  const float k1 = kLog2e, kt = kLog2e * rtau, b1 = -m * k1, bt = -m * kt;
   const bool hard = has_label && alpha != 1.f, soft = tm > -INFINITY && alpha != 0.f;
-  const bool same = tau == 1.f;
-
-  float sums[4] = {0.f, 0.f, 0.f, 0.f};              // z1, ztau, zq, sum e_k (log e_k - x_k / tau)
-  auto add = [&](const float (&f)[N]) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float d = f[j] - m;
-      const float e1 = __builtin_amdgcn_exp2f(d * k1);
-      sums[0] += e1;
-      sums[1] += same ? e1 : __builtin_amdgcn_exp2f(d * kt);
-    }
-  };
-  if constexpr (NCH > 0) {
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      float f[N];
-      forget(keep[i]);
-      R::get(keep[i], f);
-      add(f);
-    }
-  } else {
-    for (int c = tid; c < chunks; c += NT) {
-      float f[N];
-      fetch(c, f);
-      add(f);
-    }
+  char* const g = (char*)a.grad + row * (int64_t)V * R::SIZE;
+  if (!hard && !soft) {                              // no loss and no gradient, whatever the logits are
+    if (tid == 0 && a.row_loss) a.row_loss[row] = 0.f;
+    if (!a.grad) return;
+    u32x4 zero = {0, 0, 0, 0};
+    for (int c = tid; c < full; c += NT) ((C*)g)[c].v = zero;
+    if (tid < V - full * N) R::store(g, full * N + tid, 0.f);
+    return;
   }
+  float sums[4] = {0.f, 0.f, 0.f, 0.f};            // z1, ztau, zq, sum e_k (log e_k - x_k / tau)
+  auto add = [&](float v) {
+    sums[0] += __builtin_amdgcn_exp2f(fmaf(v, k1, b1));
+    sums[1] += __builtin_amdgcn_exp2f(fmaf(v, kt, bt));
+  };
+  each([&](int, const float (&f)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) add(f[j]);
+  });
+  add(more);
   if (soft)
     for (int k = tid; k < K; k += NT) {
       const float d = (s_e[k] - tm) * rtau;
@@ -236,65 +228,40 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(DistillArgs a) {
   const float h1 = hard ? scale * (1.f - alpha) : 0.f, ht = soft ? scale * alpha * tau : 0.f;
   const float c1 = hard ? h1 / sums[0] : 0.f, ct = soft ? ht / sums[1] : 0.f;
   auto dense = [&](float v) {
-    const float d = v - m;
-    const float e1 = __builtin_amdgcn_exp2f(d * k1);
-    const float et = same ? e1 : __builtin_amdgcn_exp2f(d * kt);
-    return c1 * e1 + ct * et;
+    return fmaf(c1, __builtin_amdgcn_exp2f(fmaf(v, k1, b1)), ct * __builtin_amdgcn_exp2f(fmaf(v, kt, bt)));
   };
-  // the corrected places: their logits are read before any gradient is written (the gradient may
-  // be written over the logits)
-  float late = 0.f;
-  const int entries = K + 1;                          // the teacher's, then the label
+  // The corrected places, each computed by the entries that have it (the teacher's, then the
+  // label).  Their logits are read before any gradient is written: it may take the logits' place.
+  const int entries = K + 1;
   auto place = [&](int k) { return k < K ? s_idx[k] : (has_label ? y : -1); };
-  auto value = [&](int i, float xi) {
-    float off = has_label && i == y ? h1 : 0.f;
-    if (soft) {
-      float q = 0.f;
-      for (int k = 0; k < K; ++k) q += s_idx[k] == i ? s_e[k] : 0.f;
-      off += ht * (q / sums[2]);
-    }
-    return dense(xi) - off;
-  };
-  // (hard or soft: a row with neither has no gradient, whatever its logits are)
-  const bool any = hard || soft;
+  float late = 0.f;
+  float* const lates = lds + 2 * K + 4 * (NT / 64);  // [K] where there are more entries than threads
   for (int k = tid; k < entries; k += NT) {
     const int i = place(k);
-    if (i >= 0 && any) late = value(i, R::load(x, i));
-    if (K >= NT && k < K) lds[2 * K + 4 * (NT / 64) + k] = late;   // more entries than threads
+    if (i >= 0) {
+      float off = has_label && i == y ? h1 : 0.f;
+      if (soft) {
+        float q = 0.f;
+        for (int n = 0; n < K; ++n) q += s_idx[n] == i ? s_e[n] : 0.f;
+        off += ht * (q / sums[2]);
+      }
+      late = dense(R::load(x, i)) - off;
+    }
+    if (K >= NT && k < K) lates[k] = late;
   }
   __syncthreads();
-  char* g = (char*)a.grad + row * (int64_t)V * R::SIZE;
-  auto emit = [&](int c, const float (&f)[N]) {
+  // (written past the caches: nothing here reads it again, and what the next rows read stays)
+  each([&](int c, const float (&f)[N]) {
     float o[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) o[j] = any ? dense(f[j]) : 0.f;
-    if ((c + 1) * N <= V) {
-      ((C*)g)[c].v = R::put(o);
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (c * N + j < V) R::store(g, c * N + j, o[j]);
-    }
-  };
-  if constexpr (NCH > 0) {
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      float f[N];
-      forget(keep[i]);
-      R::get(keep[i], f);
-      emit(i * NT + tid, f);
-    }
-  } else {
-    for (int c = tid; c < chunks; c += NT) {
-      float f[N];
-      fetch(c, f);
-      emit(c, f);
-    }
-  }
+    for (int j = 0; j < N; ++j) o[j] = dense(f[j]);
+    if (c + tid < full) __builtin_nontemporal_store(R::put(o), &((C*)(g + c * 16))[tid].v);
+  });
+  if (tid < V - full * N) R::store(g, full * N + tid, dense(more));
   __syncthreads();
   for (int k = tid; k < entries; k += NT) {
     const int i = place(k);
-    if (i >= 0 && any) R::store(g, i, K >= NT && k < K ? lds[2 * K + 4 * (NT / 64) + k] : late);
+    if (i >= 0) R::store(g, i, K >= NT && k < K ? lates[k] : late);
   }
 }
 
@@ -315,25 +282,25 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
   }
 }
 
-template <class E, int NT, int NCH>
+template <class E, int NT, int NCH, int WAVES>
 void launch(const DistillArgs& a, int rows, hipStream_t st) {
   const size_t lds = 4 * (2 * (size_t)a.K + 4 * (NT / 64) + (a.K >= NT ? a.K : 0));
-  hipLaunchKernelGGL((distill_row_kernel<E, NT, NCH>), dim3(rows), dim3(NT), lds, st, a);
+  hipLaunchKernelGGL((distill_row_kernel<E, NT, NCH, WAVES>), dim3(rows), dim3(NT), lds, st, a);
 }
 
-// The smallest group of threads that holds the row in 8 chunks each; 1024 threads hold 16; what
-// is longer is read again in each pass.
+// Threads of a row and the chunks that each holds.  Small groups: several rows of a CU then load,
+// add up and write at different times (32000 bf16 logits: 16 chunks of 256 threads 874 us, 8 of 512
+// 896, 4 of 1024 1929; 49999 f32 logits: 25 of 512 80 us, 16 of 1024 103).
 template <class E>
 void choose(const DistillArgs& a, int rows, hipStream_t st) {
   const int chunks = (a.V + Row<E>::N - 1) / Row<E>::N;
-  if (chunks <= 256) launch<E, 256, 1>(a, rows, st);
-  else if (chunks <= 512) launch<E, 256, 2>(a, rows, st);
-  else if (chunks <= 1024) launch<E, 256, 4>(a, rows, st);
-  else if (chunks <= 2048) launch<E, 256, 8>(a, rows, st);
-  else if (chunks <= 4096) launch<E, 512, 8>(a, rows, st);
-  else if (chunks <= 8192) launch<E, 1024, 8>(a, rows, st);
-  else if (chunks <= 16384) launch<E, 1024, 16>(a, rows, st);
-  else launch<E, 1024, 0>(a, rows, st);
+  if (chunks <= 512) launch<E, 256, 2, 4>(a, rows, st);
+  else if (chunks <= 2048) launch<E, 256, 8, 4>(a, rows, st);
+  else if (chunks <= 4096) launch<E, 256, 16, 4>(a, rows, st);
+  else if (chunks <= 8192) launch<E, 512, 16, 4>(a, rows, st);
+  else if (chunks <= 512 * 25) launch<E, 512, 25, 4>(a, rows, st);
+  else if (chunks <= 1024 * 16) launch<E, 1024, 16, 4>(a, rows, st);
+  else launch<E, 1024, 0, 4>(a, rows, st);
 }
 
 }  // namespace

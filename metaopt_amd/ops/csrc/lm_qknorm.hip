@@ -114,40 +114,29 @@ struct QkBwdArgs {
   float eps;
 };
 
-// One block: rows [per * blockIdx.x, ...) of trial blockIdx.y; its sums of dw over rows and heads
-// go to part in a fixed order (no atomics), qk_norm_dw_kernel adds the blocks.
+// `heads` query or key heads of rows [r0, r0 + n), the first at column c0 of x: their dx, and this
+// thread's terms of dw
 template <class E, int D, bool IL>
-__global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(QkBwdArgs a) {
+__device__ __forceinline__ void heads_bwd(const QkBwdArgs& a, int r0, int n, int c0, int heads, const uint16_t* dz,
+                                          const uint16_t* wg, float (&acc)[8]) {
   constexpr int LPR = D / 8, UPB = 256 / LPR;
-  __shared__ float red[UPB][2 * D + 4];
-  const int nh = a.H + 2 * a.KV;
-  const int col = (threadIdx.x % LPR) * 8, slot = threadIdx.x / LPR;
-  const int lo = blockIdx.x * a.per, hi = min(lo + a.per, a.rpt);
-  const int p = blockIdx.y;
-  float wq[8], wk[8], aq[8] = {}, ak[8] = {};
-  up8<E>(*(const u32x4*)(a.wq + (int64_t)p * D + col), wq);
-  up8<E>(*(const u32x4*)(a.wk + (int64_t)p * D + col), wk);
-  const int units = (hi - lo) * nh;
-  for (int u = slot; u < units; u += UPB) {
-    const int rl = u / nh, hh = u - rl * nh;
-    const int r = p * a.rpt + lo + rl;
+  const int nh = a.H + 2 * a.KV, col = (threadIdx.x % LPR) * 8;
+  float w[8];
+  up8<E>(*(const u32x4*)(wg + col), w);
+  const int units = n * heads;
+#pragma unroll 2
+  for (int u = threadIdx.x / LPR; u < units; u += UPB) {
+    const int rl = u / heads, hh = u - rl * heads, r = r0 + rl;
     const int b = r / a.T, t = r - b * a.T;
-    uint16_t* dst = a.dx + ((int64_t)r * nh + hh) * D + col;
-    if (hh >= a.H + a.KV) {
-      *(u32x4*)dst = *(const u32x4*)(a.dv + (((int64_t)b * a.KV + hh - a.H - a.KV) * a.T + t) * D + col);
-      continue;
-    }
-    const bool isq = hh < a.H;
     float x[8], d[8];
-    up8<E>(*(const u32x4*)(a.x + (int64_t)r * a.x_ld + hh * D + col), x);
-    up8<E>(*(const u32x4*)(isq ? a.dq + (((int64_t)b * a.H + hh) * a.T + t) * D + col
-                               : a.dk + (((int64_t)b * a.KV + hh - a.H) * a.T + t) * D + col), d);
+    up8<E>(*(const u32x4*)(a.x + (int64_t)r * a.x_ld + c0 + hh * D + col), x);
+    up8<E>(*(const u32x4*)(dz + (((int64_t)b * heads + hh) * a.T + t) * D + col), d);
     rotate8<D, IL>(d, a.cosT + (int64_t)t * (D / 2), a.sinT + (int64_t)t * (D / 2), col, -1.f);
     float ss = 0.f, dot = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       ss = fmaf(x[j], x[j], ss);
-      dot = fmaf(d[j] * (isq ? wq[j] : wk[j]), x[j], dot);
+      dot = fmaf(d[j] * w[j], x[j], dot);
     }
     ss = sum_lanes<LPR>(ss);
     dot = sum_lanes<LPR>(dot);
@@ -155,12 +144,30 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(QkBwdArgs a) {
     float o[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      o[j] = rstd * (d[j] * (isq ? wq[j] : wk[j]) - x[j] * m);
-      const float g = d[j] * x[j] * rstd;
-      aq[j] += isq ? g : 0.f;
-      ak[j] += isq ? 0.f : g;
+      o[j] = rstd * (d[j] * w[j] - x[j] * m);
+      acc[j] += d[j] * x[j] * rstd;
     }
-    *(u32x4*)dst = down8<E>(o);
+    *(u32x4*)(a.dx + ((int64_t)r * nh) * D + c0 + hh * D + col) = down8<E>(o);
+  }
+}
+
+// One block: rows [per * blockIdx.x, ...) of trial blockIdx.y; its sums of dw over rows and heads
+// go to part in a fixed order (no atomics), qk_norm_dw_kernel adds the blocks.
+template <class E, int D, bool IL>
+__global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(QkBwdArgs a) {
+  constexpr int LPR = D / 8, UPB = 256 / LPR;
+  __shared__ float red[UPB][2 * D + 4];
+  const int col = (threadIdx.x % LPR) * 8, slot = threadIdx.x / LPR, p = blockIdx.y;
+  const int lo = blockIdx.x * a.per, n = min(lo + a.per, a.rpt) - lo, r0 = p * a.rpt + lo;
+  float aq[8] = {}, ak[8] = {};
+  heads_bwd<E, D, IL>(a, r0, n, 0, a.H, a.dq, a.wq + (int64_t)p * D, aq);
+  heads_bwd<E, D, IL>(a, r0, n, a.H * D, a.KV, a.dk, a.wk + (int64_t)p * D, ak);
+  const int units = n * a.KV, nh = a.H + 2 * a.KV;
+#pragma unroll 2
+  for (int u = slot; u < units; u += UPB) {            // values: copied
+    const int rl = u / a.KV, hh = u - rl * a.KV, r = r0 + rl, b = r / a.T, t = r - b * a.T;
+    *(u32x4*)(a.dx + ((int64_t)r * nh + a.H + a.KV + hh) * D + col) =
+        *(const u32x4*)(a.dv + (((int64_t)b * a.KV + hh) * a.T + t) * D + col);
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -241,22 +248,14 @@ int mopt_qk_norm_rope_fwd(const void* x, int64_t x_ld, const void* wq, const voi
   return D == 64 ? fwd<Fp16, 64>(a, il, st) : fwd<Fp16, 128>(a, il, st);
 }
 
-// blocks of a trial's rows (part holds [P][blocks][2][D] floats)
-int mopt_qk_norm_rope_blocks(int rpt, int P, int nh, int D) {
-  const int64_t units = (int64_t)rpt * nh * D / 2048;       // block steps of one trial
-  int64_t n = (1024 + P - 1) / P;                           // 4 blocks a CU over all trials
-  if (n > (units + 3) / 4) n = (units + 3) / 4;             // at least 4 steps each
-  if (n > rpt) n = rpt;
-  return n < 1 ? 1 : (int)n;
-}
-
+// blocks: workgroups of each trial's rows; part: workspace of [P][blocks][2][D] floats
 int mopt_qk_norm_rope_bwd(const void* x, int64_t x_ld, const void* wq, const void* wk,
                           const void* cosT, const void* sinT, const void* dq, const void* dk,
                           const void* dv, void* dx, void* part, void* dwq, void* dwk, int rows, int T,
-                          int H, int KV, int rpt, int D, float eps, int il, int dtype, void* stream) {
-  if (rows <= 0 || T <= 0 || H <= 0 || KV <= 0 || rpt <= 0 || rows % rpt || (D != 64 && D != 128)) return 1;
+                          int H, int KV, int rpt, int D, int blocks, float eps, int il, int dtype,
+                          void* stream) {
+  if (rows <= 0 || T <= 0 || H <= 0 || KV <= 0 || rpt <= 0 || rows % rpt || blocks <= 0 || blocks > rpt || (D != 64 && D != 128)) return 1;
   const int P = rows / rpt;
-  int blocks = mopt_qk_norm_rope_blocks(rpt, P, H + 2 * KV, D);
   const int per = (rpt + blocks - 1) / blocks;
   if ((int64_t)per * (H + 2 * KV) >= (1ll << 31) - 256) return 1;
   const QkBwdArgs a{(const uint16_t*)x, x_ld, (const uint16_t*)wq, (const uint16_t*)wk,

@@ -9,7 +9,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .heads import _call, _p, _same
+from .heads import _call, _once, _p, _same
 from .lm import _hip, _ScaledGrad
 
 c_void_p, c_int, c_float, c_int64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
@@ -80,8 +80,7 @@ class _Distill(torch.autograd.Function):
                     alpha if not torch.is_tensor(alpha) else None, rows_per_trial, scale)
         return _launch(logits, labels, top, index, tau, alpha, rows_per_trial, scale, None, None, True)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dloss):
         if ctx.unit:
             (grad,) = ctx.saved_tensors
@@ -103,7 +102,7 @@ def _mix(name, v, P, like, low, high):
                              "one a trial")
         if v.requires_grad:
             raise ValueError(f"{name} has no gradient here: detach it")
-        _same(like, {name: v})
+        _same(like, name, v)
         return v
     v = float(v)
     if not low <= v <= high:
@@ -147,7 +146,7 @@ def distill_loss(logits, labels, top_values, top_index, rows_per_trial, temperat
         raise ValueError("the teacher has no gradient here: detach top_values")
     if inplace and not unit_weights:
         raise ValueError("inplace needs unit_weights: the backward reads the logits again")
-    _same(logits, {"labels": labels, "top_values": top_values, "top_index": top_index})
+    _same(logits, "labels top_values top_index", labels, top_values, top_index)
     P = R // rows_per_trial
     tau = _mix("temperature", temperature, P, logits, 1e-6, 1e6)
     alpha = _mix("alpha", alpha, P, logits, 0.0, 1.0)

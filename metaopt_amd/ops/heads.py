@@ -24,8 +24,7 @@ c_void_p, c_int, c_float, c_int64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_floa
 _lib.register_signatures({
     "mopt_qk_norm_rope_fwd": ([c_void_p, c_int64] + [c_void_p] * 9 + [c_int] * 8 +
                               [c_float, c_int, c_int, c_void_p], c_int),
-    "mopt_qk_norm_rope_blocks": ([c_int] * 4, c_int),
-    "mopt_qk_norm_rope_bwd": ([c_void_p, c_int64] + [c_void_p] * 11 + [c_int] * 6 +
+    "mopt_qk_norm_rope_bwd": ([c_void_p, c_int64] + [c_void_p] * 11 + [c_int] * 7 +
                               [c_float, c_int, c_int, c_void_p], c_int),
     "mopt_window_fwd": ([c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int] * 8 +
                         [c_float, c_int, c_void_p], c_int),
@@ -43,12 +42,14 @@ MAX_LENGTH = 1 << 29
 def _call(t: torch.Tensor, name: str, *args) -> None:
     """Launch on the current stream of ``t``'s device, whichever device is current."""
     fn = getattr(_lib.get_lib(), name)
-    if t.device.index not in (None, torch.cuda.current_device()):
-        with torch.cuda.device(t.device):
+    index = t.get_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             rc = fn(*args, _lib.stream_ptr(t.device))
     else:
-        rc = fn(*args, _lib.stream_ptr(t.device))
-    _lib.check(rc, name)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc or _lib.SYNC_CHECK:
+        _lib.check(rc, name)
 
 
 def _p(t: Optional[torch.Tensor]):
@@ -67,10 +68,20 @@ def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
-def _same(t: torch.Tensor, others: dict) -> None:
-    for name, o in others.items():
-        if o.device != t.device:
-            raise ValueError(f"{name} is on {o.device}, the input on {t.device}")
+def _same(t: torch.Tensor, names: str, *others) -> None:
+    device = t.device
+    for i, o in enumerate(others):
+        if o.device != device:
+            raise ValueError(f"{names.split()[i]} is on {o.device}, the input on {device}")
+
+
+def _once(backward):
+    """``once_differentiable`` at the price of one test where no graph of the backward is asked for."""
+    strict = torch.autograd.function.once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return strict(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return staticmethod(call)
 
 
 def _int32(name: str, t: torch.Tensor, n: int) -> None:
@@ -134,7 +145,7 @@ def _check_qk(qkv, wq, wk, cos, sin, T, H, KV):
             raise ValueError(f"{name} has no gradient here: detach it")
     if not (wq.dtype == wk.dtype == qkv.dtype):
         raise ValueError("qkv, wq and wk must be of one type")
-    _same(qkv, {"wq": wq, "wk": wk, "cos": cos, "sin": sin})
+    _same(qkv, "wq wk cos sin", wq, wk, cos, sin)
     if D % 2:
         raise ValueError(f"head dimension {D}: pairs are rotated")
     return P, D, R
@@ -158,18 +169,27 @@ def _qk_fwd(qkv, wq, wk, cos, sin, T, H, KV, eps, il, k, v, start, cap):
     return q
 
 
+def _qk_blocks(rows: int, P: int, columns: int) -> int:
+    """Workgroups of the backward for each trial's ``rows``: 8 a CU over all trials, each with 4 steps
+    (of 2048 values) at least."""
+    return max(1, min(-(-2048 // P), -(-rows * columns // 8192), rows))
+
+
+def _qk_heads(qkv, wq, wk, cos, sin, T, H, KV, eps, il):
+    shape = qkv.shape[0] // T, KV, T, wq.shape[1]
+    k = torch.empty(shape, dtype=qkv.dtype, device=qkv.device)
+    v = torch.empty_like(k)
+    return _qk_fwd(qkv, wq, wk, cos, sin, T, H, KV, eps, il, k, v, None, T), k, v
+
+
 class _QKNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, wq, wk, cos, sin, T, H, KV, eps, il):
-        k, v = (torch.empty(qkv.shape[0] // T, KV, T, wq.shape[1], dtype=qkv.dtype,
-                            device=qkv.device) for _ in range(2))
-        q = _qk_fwd(qkv, wq, wk, cos, sin, T, H, KV, eps, il, k, v, None, T)
         ctx.save_for_backward(qkv, wq, wk, cos, sin)
         ctx.meta = (T, H, KV, eps, il)
-        return q, k, v
+        return _qk_heads(qkv, wq, wk, cos, sin, T, H, KV, eps, il)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dq, dk, dv):
         qkv, wq, wk, cos, sin = ctx.saved_tensors
         T, H, KV, eps, il = ctx.meta
@@ -177,13 +197,13 @@ class _QKNormRope(torch.autograd.Function):
         dx = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         if R == 0:
             return (dx, torch.zeros_like(wq), torch.zeros_like(wk)) + (None,) * 7
-        dq, dk, dv = (_dense16(t) for t in (dq, dk, dv))
+        dq, dk, dv = _dense16(dq), _dense16(dk), _dense16(dv)
         dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
-        blocks = _lib.get_lib().mopt_qk_norm_rope_blocks(R // P, P, H + 2 * KV, D)
+        blocks = _qk_blocks(R // P, P, (H + 2 * KV) * D)
         part = torch.empty(P * blocks * 2 * D, dtype=torch.float32, device=qkv.device)
         _call(qkv, "mopt_qk_norm_rope_bwd", _p(qkv), qkv.stride(0), _p(wq), _p(wk), _p(cos), _p(sin),
-              _p(dq), _p(dk), _p(dv), _p(dx), _p(part), _p(dwq), _p(dwk), R, T, H, KV, R // P, D, eps,
-              int(il), _TYPES[qkv.dtype])
+              _p(dq), _p(dk), _p(dv), _p(dx), _p(part), _p(dwq), _p(dwk), R, T, H, KV, R // P, D,
+              blocks, eps, int(il), _TYPES[qkv.dtype])
         return (dx, dwq, dwk) + (None,) * 7
 
 
@@ -207,11 +227,10 @@ def qk_norm_rope(qkv, wq, wk, cos, sin, T, H, kv_heads=None, eps=1e-5, il=False)
     if not _hip(qkv, "qk_norm_rope"):
         return qk_norm_rope_ref(qkv, wq, wk, cos, sin, T, H, KV, eps, il)
     _check_kernel("qk_norm_rope", qkv, D)
-    return _QKNormRope.apply(_rows16(qkv), _dense16(wq), _dense16(wk), cos, sin, T, H, KV,
-                             float(eps), bool(il))
+    args = _rows16(qkv), _dense16(wq), _dense16(wk), cos, sin, T, H, KV, float(eps), bool(il)
+    return _QKNormRope.apply(*args) if _needs_grad(qkv, wq, wk) else _qk_heads(*args)
 
 
-@torch.no_grad()
 def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=1e-5, il=False):
     """:func:`qk_norm_rope` of the next ``T`` tokens of every sequence: sequence b's stand at
     positions ``start[b] ... start[b] + T - 1`` (int32 ``[B']``, on the device), their keys and
@@ -228,18 +247,10 @@ def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=
         raise ValueError(f"the caches are {tuple(kcache.shape)}: {n} sequences of heads of {D}")
     if kcache.dtype != qkv.dtype or vcache.dtype != qkv.dtype:
         raise ValueError("the caches must be of qkv's type")
-    _same(qkv, {"kcache": kcache, "vcache": vcache, "start": start})
+    _same(qkv, "kcache vcache start", kcache, vcache, start)
     _int32("start", start, n)
     if not _hip(qkv, "qk_norm_rope"):
-        at = start.long()[:, None] + torch.arange(T, device=qkv.device)
-        ok = (at >= 0) & (at < min(cap, cos.shape[0]))
-        part = [torch.where(ok, at, torch.zeros_like(at))]
-        f = qk_norm_rope_ref(qkv, wq, wk, _at(cos, part[0]), _at(sin, part[0]), T, H, KV, eps, il,
-                             start=torch.arange(n, device=qkv.device) * T)
-        b, t = ok.nonzero(as_tuple=True)
-        kcache[b, :, at[b, t]] = f[1][b, :, t]
-        vcache[b, :, at[b, t]] = f[2][b, :, t]
-        return f[0] * ok[:, None, :, None]
+        return _cached_ref(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps, il)
     _check_kernel("qk_norm_rope_cached", qkv, D)
     for name, c in (("kcache", kcache), ("vcache", vcache)):
         if c.stride(3) != 1 or c.data_ptr() % 16 or any(s % 8 for s in c.stride()[:3]):
@@ -251,9 +262,18 @@ def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=
                    kcache, vcache, start, cap)
 
 
-def _at(table, at):
-    """Table rows of the positions ``at`` [n, T], one after the other."""
-    return table[at.reshape(-1)]
+@torch.no_grad()
+def _cached_ref(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps, il):
+    n, KV, cap = kcache.shape[:3]
+    at = start.long()[:, None] + torch.arange(T, device=qkv.device)
+    ok = (at >= 0) & (at < min(cap, cos.shape[0]))
+    rows = torch.where(ok, at, torch.zeros_like(at)).reshape(-1)     # the tables' rows, one a token
+    q, k, v = qk_norm_rope_ref(qkv, wq, wk, cos[rows], sin[rows], T, H, KV, eps, il,
+                               start=torch.arange(n, device=qkv.device) * T)
+    b, t = ok.nonzero(as_tuple=True)
+    kcache[b, :, at[b, t]] = k[b, :, t]
+    vcache[b, :, at[b, t]] = v[b, :, t]
+    return q * ok[:, None, :, None]
 
 
 # ============================================================================ window attention
@@ -334,8 +354,7 @@ class _WindowAttention(torch.autograd.Function):
         ctx.meta = (window, sinks, scale, start0)
         return o
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, do):
         q, k, v, o, rest, lse, start, lengths = ctx.saved_tensors
         window, sinks, scale, start0 = ctx.meta
@@ -392,18 +411,18 @@ def window_attention(q, k, v, window: Optional[int] = None, sinks: int = 0, scal
         raise ValueError(f"scale {scale} must be positive")
     if max(Tq, Tk) > MAX_LENGTH:
         raise ValueError(f"sequences and caches hold at most {MAX_LENGTH} tokens")
-    _same(q, {"k": k, "v": v})
+    _same(q, "k v", k, v)
     start0 = Tk - Tq
     if torch.is_tensor(start):
         _int32("start", start, B)
-        _same(q, {"start": start})
+        _same(q, "start", start)
     elif start is not None:
         start0, start = int(start), None
         if abs(start0) > MAX_LENGTH:
             raise ValueError(f"start {start0} is no position")
     if lengths is not None:
         _int32("lengths", lengths, B)
-        _same(q, {"lengths": lengths})
+        _same(q, "lengths", lengths)
     if not _hip(q, "window_attn"):
         return window_attention_ref(q, k, v, window, sinks, scale, start0 if start is None else start,
                                     lengths)
