@@ -69,16 +69,22 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(
 // in one register; columns change it by an exclusive or, rows by an offset of the instruction.
 template <int D>
 struct Place {
-  uint32_t f, t;
+  uint32_t f, t, b;
   __device__ __forceinline__ explicit Place(int lane) {
     const int r = swap23(lane & 31), g = lane >> 4, i = lane & 15, q = 8 * (g >> 1) + (i >> 2);
     f = r * D * 2 + (((lane >> 5) ^ swz<D>(r)) << 4);
+    b = (lane & 31) * D * 2 + (((lane >> 5) ^ swz<D>(lane & 31)) << 4);
     t = q * D * 2 + (((2 * (g & 1) + ((i & 3) >> 1)) ^ swz<D>(q)) << 4) + (i & 1) * 8;
   }
   // A operand of rows [r0, r0 + 32) (r0 a multiple of 32) in the exchanged order, columns 16 ks ...
   __device__ __forceinline__ u32x4 frag(uint32_t tile, int r0, int ks) const {
     typedef __attribute__((address_space(3))) const u32x4 vec;
     return *(vec*)(uintptr_t)(((tile + f) ^ (ks << 5)) + r0 * D * 2);
+  }
+  // B operand of step ks of the 32 rows of an image: this lane's row, columns 16 ks + 8 (l >> 5) ...
+  __device__ __forceinline__ u32x4 frag_b(uint32_t image, int ks) const {
+    typedef __attribute__((address_space(3))) const u32x4 vec;
+    return *(vec*)(uintptr_t)((image + b) ^ (ks << 5));
   }
   // A operand of the transpose: rows = columns [32 dn, 32 dn + 32) of the tile, k = rows r0 ... + 15
   // (r0 a multiple of 16); rows 4 further have bit 0 of their exchange turned
@@ -116,7 +122,7 @@ __device__ __forceinline__ f32x16 zero16() {
 // 16 l ... of 1 KB), so the exchange of chunks is applied to the addresses that are read.  A ring of
 // NS tiles is filled NS - 1 ahead with one barrier a tile: the fills go through inline asm, where
 // the compiler does not see them and would wait for all of them before every transposing read, and
-// tile_wait waits for those of the next tile itself.  Rows outside [lo, hi) are read as the nearest
+// wait_barrier waits for those of the next tile itself.  Rows outside [lo, hi) are read as the nearest
 // row inside (values of the sequence, finite as the others; the masks leave them out): what padding
 // holds is never read.
 __device__ __forceinline__ uint32_t lds_at(const void* p) { return __builtin_amdgcn_readfirstlane(lds_addr(p)); }
@@ -160,9 +166,9 @@ __device__ __forceinline__ void fill_tile(const uint16_t* g, int64_t ld, int row
 }
 
 // waves a SIMD (registers: 512 / waves) and ring of a kernel (tiles of two matrices)
+template <int D> constexpr int kDkvWaves = D == 64 ? 3 : 2;
 template <int D> constexpr int kFwdWaves = D == 64 ? 4 : 2;
 template <int D> constexpr int kDqWaves = D == 64 ? 3 : 2;
-template <int D> constexpr int kDkvWaves = D == 64 ? 3 : 2;
 template <int D> constexpr int kFwdRing = 2;
 template <int D> constexpr int kBwdRing = D == 64 ? 3 : 2;
 
@@ -252,6 +258,20 @@ __device__ __forceinline__ int sight(int k0, int i0, int i1, int W, int S) {
   return 1;
 }
 
+// x of the keys k0 ... that the query at position i does not see: `with`
+template <class E>
+__device__ __forceinline__ void hide(f32x16& x, float with, int i, int k0, int lane, int W, int S) {
+  const int d0 = i - k0 - 8 * (lane >> 5);
+  if (k0 >= S) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = (uint32_t)(d0 - row_of(r, 0)) < (uint32_t)W ? x[r] : with;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      x[r] = (uint32_t)(d0 - row_of(r, 0)) < (k0 + row_of(r, lane) < S ? 1u << 31 : (uint32_t)W) ? x[r] : with;
+  }
+}
+
 template <class E, int D>
 __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a, uint16_t* o, uint16_t* rest,
                                                                        float* lse) {
@@ -298,32 +318,23 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
       if (it + NS - 1 < tiles.n) fetch(it + NS - 1);
       const uint32_t Ks = lds_at(ring[(it + 1) % NS][0]), Vs = lds_at(ring[(it + 1) % NS][1]);
       if (wt0 > wt1) continue;
-#pragma unroll 1
-      for (int sub = 0; sub < 2; ++sub) {
-        const int k0 = tiles.key(it) + 32 * sub;
-        const int see = sight(k0, s.st + wt0, s.st + wt1, a.W, a.S);
-        if (see == 0) continue;
+      // products of the scores of a group of 32 keys, their maximum, their exponentials and P V
+      auto scores = [&](int sub) {
         f32x16 x = zero16();
 #pragma unroll
         for (int ks = 0; ks < DK; ++ks) x = E::mfma32(at.frag(Ks + sub * 64 * D, 0, ks), qf[ks], x);
-        if (see == 1) {
-          const int d0 = i - k0 - 8 * (lane >> 5);
-          if (k0 >= a.S) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = (uint32_t)(d0 - row_of(r, 0)) < (uint32_t)a.W ? x[r] : -INFINITY;
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              x[r] = (uint32_t)(d0 - row_of(r, 0)) < (k0 + row_of(r, lane) < a.S ? 1u << 31 : (uint32_t)a.W)
-                         ? x[r] : -INFINITY;
-          }
-        }
+        return x;
+      };
+      auto most = [&](const f32x16& x) {
         float mx = x[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
+        return mx;
+      };
+      // the reference of the exponents moves only when a row's maximum has grown past 2^8 of it:
+      // sums and products stay far inside 32 bits, and most tiles need no rescaling
+      auto refer = [&](float mx) {
         mx = other_half(mx, true) * a.c;
-        // the reference of the exponents moves only when a row's maximum has grown past 2^8 of it:
-        // sums and products stay far inside 32 bits, and most tiles need no rescaling
         if (__any(mx > m + 8.f)) {
           const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - mn);
           m = mn;
@@ -331,6 +342,8 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
 #pragma unroll
           for (int dn = 0; dn < DN; ++dn) acc[dn] *= f;
         }
+      };
+      auto weigh = [&](f32x16& x, int sub) {
         float part = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -345,6 +358,15 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
           for (int dn = 0; dn < DN; ++dn)
             acc[dn] = E::mfma32(at.frag_t(Vs + sub * 64 * D, 16 * st, dn), p, acc[dn]);
         }
+      };
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const int k0 = tiles.key(it) + 32 * sub, see = sight(k0, s.st + wt0, s.st + wt1, a.W, a.S);
+        if (see == 0) continue;
+        f32x16 x = scores(sub);
+        if (see == 1) hide<E>(x, -INFINITY, i, k0, lane, a.W, a.S);
+        refer(most(x));
+        weigh(x, sub);
       }
     }
   }
@@ -433,31 +455,19 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
       if (it + NS - 1 < tiles.n) fetch(it + NS - 1);
       const uint32_t Ks = lds_at(ring[(it + 1) % NS][0]), Vs = lds_at(ring[(it + 1) % NS][1]);
       if (wt0 > wt1) continue;
-#pragma unroll 1
-      for (int sub = 0; sub < 2; ++sub) {
-        const int k0 = tiles.key(it) + 32 * sub;
-        const int see = sight(k0, s.st + wt0, s.st + wt1, a.W, a.S);
-        if (see == 0) continue;
-        f32x16 x = zero16(), y = zero16();
+      auto scores = [&](int sub, f32x16& x, f32x16& y) {
+        x = y = zero16();
 #pragma unroll
         for (int ks = 0; ks < DK; ++ks) {
           x = E::mfma32(at.frag(Ks + sub * 64 * D, 0, ks), qf[ks], x);
           y = E::mfma32(at.frag(Vs + sub * 64 * D, 0, ks), df[ks], y);
         }
+      };
+      auto slope = [&](f32x16& x, const f32x16& y) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.c, -ls)) * (y[r] - ds);
-        if (see == 1) {
-          const int d0 = i - k0 - 8 * (lane >> 5);
-          if (k0 >= a.S) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = (uint32_t)(d0 - row_of(r, 0)) < (uint32_t)a.W ? x[r] : 0.f;
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              x[r] = (uint32_t)(d0 - row_of(r, 0)) < (k0 + row_of(r, lane) < a.S ? 1u << 31 : (uint32_t)a.W)
-                         ? x[r] : 0.f;
-          }
-        }
+      };
+      auto add = [&](const f32x16& x, int sub) {
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
           const u32x4 p = pack<E>(x, st);
@@ -465,6 +475,16 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
           for (int dn = 0; dn < DN; ++dn)
             acc[dn] = E::mfma32(at.frag_t(Ks + sub * 64 * D, 16 * st, dn), p, acc[dn]);
         }
+      };
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const int k0 = tiles.key(it) + 32 * sub, see = sight(k0, s.st + wt0, s.st + wt1, a.W, a.S);
+        if (see == 0) continue;
+        f32x16 x, y;
+        scores(sub, x, y);
+        slope(x, y);
+        if (see == 1) hide<E>(x, 0.f, i, k0, lane, a.W, a.S);
+        add(x, sub);
       }
     }
   }
@@ -474,12 +494,16 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
 }
 
 // dK, dV.  Two kinds of items:
-// near: 128 keys, 32 a wave, with the queries that have them in their window;
+// near: 128 keys, 32 a wave, with the queries that have them in their window, or one of `parts` shares
+// of these;
 // far: 32 keys, those of sinks, with `span` of the queries that have left their window behind (j < S,
 // i - j >= W) -- pairs that would leave a few workgroups with the whole length.  The four waves take
-// turns at the groups of 32 queries and their sums are added up in the end.
-// The sums of rows j < S go to `part` [slot][b, hk][S][2][D] in 32 bits (slot 0: the near ones, then a
-// slot for each span); window_sink_kernel adds the slots.
+// turns at the groups of 32 queries.
+// What is not a key's whole sum is left in 32 bits: the near sums of all rows (parts > 1) or of rows
+// j < S, [part][b, hk][rows][2][D], and the far ones behind them, [span][wave][b, hk][S][2][D];
+// window_sum_kernel adds them.  Bound by the vector work on the scores (exp2, dS, packing) between the
+// products: 125M step (64 x 12 heads, 512 tokens, window 128, 4 sinks) 90 - 104 us.  (Two waves for each
+// key, 8 a workgroup, were slower everywhere: 272 us.)
 template <class E, int D>
 struct Dkv {
   // heads of 128: 64 registers of key and value fragments beside 128 of sums leave too few for the
@@ -497,7 +521,7 @@ struct Dkv {
   const float *lse, *dsum;
   Lds& lds;
   const Seq& s;
-  int b, hk, tq_pad, tid, lane, wave;
+  int b, hk, tq_pad, lane, wave;
   Place<D> at;
   u32x4 kf[DK], vf[kValuesInLds ? 1 : DK];
   f32x16 ak[DN], av[DN];
@@ -507,30 +531,48 @@ struct Dkv {
     for (int dn = 0; dn < DN; ++dn) ak[dn] = av[dn] = zero16();
   }
 
-  // query tile it of `per` tiles a head, the first at row tb
-  __device__ __forceinline__ void fetch(int it, int per, int tb) {
-    const int G = a.H / a.KV, hq = hk * G + it / per, row0 = tb + (it % per) * QN, slot = (it + 2) % NS;
-    fill_tile<D, QN>(a.q + b * a.q_sb + hq * a.q_sh, a.q_st, row0, s.t0, s.t1, lds.ring[slot][0], wave, lane);
-    fill_tile<D, QN>(dout + ((int64_t)b * a.Tq * a.H + hq) * D, (int64_t)a.H * D, row0, s.t0, s.t1,
-                     lds.ring[slot][1], wave, lane);
+  // Where the next tile is read from: its row, and the first head's matrices and rows of statistics;
+  // kept and moved on tile by tile (a division by the tiles of a head, twice a tile, and 64-bit
+  // products were as many scalar instructions as the step has vector ones)
+  const uint16_t *qn, *on;
+  const float* sn;
+  int row_n, slot_n;
+
+  __device__ __forceinline__ void fetch(int tb, int te) {
+    fill_tile<D, QN>(qn, a.q_st, row_n, s.t0, s.t1, lds.ring[slot_n][0], wave, lane);
+    fill_tile<D, QN>(on, (int64_t)a.H * D, row_n, s.t0, s.t1, lds.ring[slot_n][1], wave, lane);
     // (waves 2 and 3 write what waves 0 and 1 do: each has the same number of loads under way)
-    fill4(scalar(((wave & 1) ? dsum : lse) + ((int64_t)b * a.H + hq) * tq_pad + row0),
-          4 * (lane & (QN - 1)), lds.stat[slot][wave & 1]);
+    fill4(scalar(sn + row_n), 4 * (lane & (QN - 1)), lds.stat[slot_n][wave & 1]);
+    slot_n = slot_n + 1 == NS ? 0 : slot_n + 1;
+    row_n += QN;
+    if (row_n >= te) {                                 // the next head's first tile
+      row_n = tb;
+      qn += a.q_sh;
+      on += D;
+      sn += tq_pad;
+    }
   }
 
-  // All tiles of rows [t0, t1) of every query head, for the pairs with lo <= i - j < lo + n: the
-  // window's (0, W), or far ones (W, as many as there may be; j < S)
-  __device__ __forceinline__ void run(bool far, int kw, int t0, int t1) {
-    const int tb = t0 & ~(QN - 1), per = (t1 - 1 - tb) / QN + 1, tiles = per * (a.H / a.KV);
+  // Tiles [it0, it1) of those of rows [tb, te) of each query head, for the pairs with
+  // lo <= i - j < lo + n: the window's (0, W), or far ones (W, as many as there may be; j < S)
+  __device__ __forceinline__ void run(bool far, int kw, int tb, int te, int it0, int it1) {
     constexpr int kTile = 2 * kFills<D, QN> + 1;
-    // the wave's keys and values: slots 0 and 1 of three; heads of 128: both slots, and the values' place
+    const int per = (te - 1 - tb) / QN + 1, skip = it0 / per, hq = hk * (a.H / a.KV) + skip;
+    int row0 = tb + (it0 - skip * per) * QN, slot = NS == 3 ? 2 : 0;
+    row_n = row0;
+    slot_n = slot;
+    qn = a.q + b * a.q_sb + hq * a.q_sh;
+    on = dout + ((int64_t)b * a.Tq * a.H + hq) * D;
+    sn = ((wave & 1) ? dsum : lse) + ((int64_t)b * a.H + hq) * tq_pad;
+    // the wave's keys and values: slots 0 and 1 of three; heads of 128: both slots, and the
+    // values' place
     uint16_t* img = lds.ring[0][0] + wave * Rows<D>::SIZE;
     uint16_t* vimg = kValuesInLds ? lds.values + wave * Rows<D>::SIZE : img + 4 * Rows<D>::SIZE;
     Rows<D>::fill(a.k + b * a.k_sb + hk * a.k_sh, a.k_st, kw, 0, s.len, img, lane);
     Rows<D>::fill(a.v + b * a.v_sb + hk * a.v_sh, a.v_st, kw, 0, s.len, vimg, lane);
-    int issued = 0;
+    int issued = it0;
     if (NS == 3) {                                     // (a tile goes into the third slot)
-      fetch(issued++, per, tb);
+      fetch(tb, te), ++issued;
       wait_own<kTile>();
     } else {
       wait_own<0>();
@@ -539,23 +581,24 @@ struct Dkv {
     if constexpr (!kValuesInLds) Rows<D>::read(vimg, vf, lane);
     if (NS == 2) {
       wait_barrier<0>();
-      fetch(issued++, per, tb);
+      fetch(tb, te), ++issued;
     }
     const int j = kw + (lane & 31), lo = far ? a.W : 0;
     const uint32_t n = far ? 1u << 30 : (uint32_t)a.W, mine = far && j >= a.S ? 0 : n;
-    for (int it = 0; it < tiles; ++it) {
+    for (int it = it0; it < it1; ++it) {
       if (issued - it - 1 == NS - 2) wait_barrier<kTile * (NS - 2)>();
       else wait_barrier<0>();
-      while (issued < min(tiles, it + NS)) fetch(issued++, per, tb);
-      const int row0 = tb + (it % per) * QN;
+      while (issued < min(it1, it + NS)) fetch(tb, te), ++issued;
 #pragma unroll 1
       for (int sub = 0; sub < SUBS; ++sub) {
         if (far && ((it * SUBS + sub) & 3) != wave) continue;
         const int least = s.st + row0 + 32 * sub - kw - 31;   // of i - j; the largest is 62 more
         if (least + 62 < lo || (least >= lo && (uint32_t)(least - lo) >= n)) continue;
         const bool all = least >= lo && (uint32_t)(least + 62 - lo) < n && (!far || kw + 31 < a.S);
-        step((it + 2) % NS, sub, all, least + 31 + kw - j - lo, mine);
+        step(slot, sub, all, least + 31 + kw - j - lo, mine);
       }
+      slot = slot + 1 == NS ? 0 : slot + 1;
+      row0 = row0 + QN >= te ? tb : row0 + QN;
     }
   }
 
@@ -580,15 +623,12 @@ struct Dkv {
       for (int r = 0; r < 16; ++r) x[r] = (uint32_t)(d + row_of(r, 0)) < mine ? x[r] : 0.f;
     }
     if (D == 128) __builtin_amdgcn_sched_barrier(0);
+    // (opaque: the places of the values would be kept over the loop, in 8 registers that it needs)
+    uint32_t values = lds_at(lds.values) + wave * Rows<D>::SIZE * 2;
+    asm volatile("" : "+v"(values));
 #pragma unroll
-    for (int ks = 0; ks < DK; ++ks) {
-      u32x4 f;
-      if constexpr (kValuesInLds)
-        f = lds16(lds.values + wave * Rows<D>::SIZE + lds_off<D>(lane & 31, 16 * ks + 8 * (lane >> 5)));
-      else
-        f = vf[ks];
-      y = E::mfma32(at.frag(Os, 0, ks), f, y);
-    }
+    for (int ks = 0; ks < DK; ++ks)
+      y = E::mfma32(at.frag(Os, 0, ks), kValuesInLds ? at.frag_b(values, ks) : vf[kValuesInLds ? 0 : ks], y);
     if constexpr (D == 128) {                          // reads two products ahead, not all at once
       __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
@@ -631,43 +671,29 @@ struct Dkv {
         *(f32x4*)(dst + D + col) = f32x4{av[dn][4 * r4], av[dn][4 * r4 + 1], av[dn][4 * r4 + 2], av[dn][4 * r4 + 3]};
       }
   }
-
-  // x of the four waves added up in wave 0, in their order
-  __device__ __forceinline__ void join(f32x16 (&x)[DN]) {
-    float* buf = (float*)&lds;                         // 3 waves, 16 DN registers, 64 lanes
-    __syncthreads();
-    if (wave)
-#pragma unroll
-      for (int dn = 0; dn < DN; ++dn)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) buf[(((wave - 1) * DN + dn) * 16 + r) * 64 + lane] = x[dn][r];
-    __syncthreads();
-    if (!wave)
-      for (int w = 0; w < 3; ++w)
-#pragma unroll
-        for (int dn = 0; dn < DN; ++dn)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x[dn][r] += buf[((w * DN + dn) * 16 + r) * 64 + lane];
-  }
 };
 
 template <class E, int D>
-__global__ __launch_bounds__(256, kDkvWaves<D>) void window_dkv_kernel(WinArgs a, const uint16_t* dout, const float* lse,
-                                                         const float* dsum, uint16_t* dk, uint16_t* dv,
-                                                         float* part, int spans, int span, float scale) {
+__global__ __launch_bounds__(256, kDkvWaves<D>) void window_dkv_kernel(
+    WinArgs a, const uint16_t* dout, const float* lse, const float* dsum, uint16_t* dk, uint16_t* dv, float* part,
+    int parts, int spans, int span, float scale) {
   using K = Dkv<E, D>;
-  static_assert(sizeof(typename K::Lds) >= 3 * 64 * D / 2 * 4, "room to join the waves");
+  constexpr int QN = K::QN;
   __shared__ __attribute__((aligned(256))) typename K::Lds lds;
-  const int nkb = (a.Tk + BM - 1) / BM;
-  const int nst = spans ? (a.S + 31) / 32 : 0, items = nkb + nst * spans;
-  const int item = xcd_remap((int)blockIdx.x, (int)gridDim.x);
-  const int bk = item / items, it0 = item - bk * items, b = bk / a.KV, hk = bk - b * a.KV;
+  const int nkb = (a.Tk + BM - 1) / BM * parts;
+  // far items come first and go round the XCDs, near ones lie together by key head (a multiple of 8
+  // before them): each XCD gets its share of both
+  const int nfar = spans ? (a.S + 31) / 32 * spans : 0, fars = nfar * a.B * a.KV, first = (fars + 7) & ~7;
+  if ((int)blockIdx.x >= fars && (int)blockIdx.x < first) return;
+  const bool far = (int)blockIdx.x < fars;
+  const int item = far ? (int)blockIdx.x : xcd_remap((int)blockIdx.x - first, (int)gridDim.x - first);
+  const int bk = item / (far ? nfar : nkb), it0 = item - bk * (far ? nfar : nkb), b = bk / a.KV, hk = bk - b * a.KV;
   const Seq s = seq_of(a, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  K k{a, dout, lse, dsum, lds, s, b, hk, (a.Tq + BM - 1) / BM * BM, tid, lane, wave, Place<D>(lane)};
-  const bool far = it0 < nst * spans;
-  const int c = far ? it0 % spans : 0;
-  const int kb = it0 - nst * spans, kw = far ? it0 / spans * 32 : kb * BM + wave * 32, j = kw + (lane & 31);
+  K k{a, dout, lse, dsum, lds, s, b, hk, (a.Tq + BM - 1) / BM * BM, lane, wave, Place<D>(lane)};
+  const int G = a.H / a.KV, c = it0 % (far ? spans : parts);
+  const int kb = it0 / parts, kw = far ? it0 / spans * 32 : kb * BM + wave * 32;
+  const int j = kw + (lane & 31);
   // near: queries of positions [kb BM, last key + W)
   int t0 = max(s.t0, kb * BM - s.st);
   int t1 = (int)min((int64_t)s.t1, (int64_t)kb * BM + BM - 1 + a.W - s.st);
@@ -676,40 +702,49 @@ __global__ __launch_bounds__(256, kDkvWaves<D>) void window_dkv_kernel(WinArgs a
     t1 = (int)min((int64_t)s.t1, (int64_t)(c + 1) * span);
   }
   k.clear();
-  if (t0 < t1 && (far ? kw : kb * BM) < s.len) k.run(far, kw, t0, t1);
+  if (t0 < t1 && (far ? kw : kb * BM) < s.len) {
+    const int tb = t0 & ~(QN - 1), per = (t1 - 1 - tb) / QN + 1, tiles = per * G;
+    const int share = far ? tiles : (tiles + parts - 1) / parts, it = far ? 0 : c * share;
+    if (it < tiles) k.run(far, kw, tb, t1, it, min(tiles, it + share));
+  }
+  const int64_t bks = (int64_t)a.B * a.KV, rows = parts > 1 ? a.Tk : a.S;
   if (far) {
-    k.join(k.ak);
-    k.join(k.av);
-    if (!wave && j < a.S) k.put_part(part + (((int64_t)(1 + c) * a.B * a.KV + bk) * a.S + j) * 2 * D);
+    if (j < a.S) k.put_part(part + (parts * bks * rows + ((c * 4 + wave) * bks + bk) * a.S + j) * 2 * D);
     return;
   }
-  const bool sink = spans && j < a.S;
-  uint16_t* img = lds.ring[0][0] + wave * Rows<D>::SIZE;
-  const int64_t base = (int64_t)bk * a.Tk * D;
-  const int lo = spans ? a.S : 0;                      // (rows of sinks: window_sink_kernel)
   __syncthreads();
-  Rows<D>::template put<E, false>(k.ak, scale, dk + base, D, kw, lo, a.Tk, img, lane);
-  Rows<D>::template put<E, false>(k.av, K::kUnshift, dv + base, D, kw, lo, a.Tk, img, lane);
-  if (sink) k.put_part(part + ((int64_t)bk * a.S + j) * 2 * D);
+  uint16_t* img = lds.ring[0][0] + wave * Rows<D>::SIZE;
+  const bool some = parts > 1 || (spans && j < a.S);    // what window_sum_kernel adds up
+  if (parts == 1) {
+    const int64_t base = (int64_t)bk * a.Tk * D;
+    const int lo = spans ? a.S : 0;
+    Rows<D>::template put<E, false>(k.ak, scale, dk + base, D, kw, lo, a.Tk, img, lane);
+    Rows<D>::template put<E, false>(k.av, K::kUnshift, dv + base, D, kw, lo, a.Tk, img, lane);
+  }
+  if (some && j < a.Tk) k.put_part(part + ((c * bks + bk) * rows + j) * 2 * D);
 }
 
-// dk, dv rows j < min(S, Tk) from the slots of window_dkv_kernel, in their order
+// dk, dv of the first `rows` rows of each key head, from what window_dkv_kernel left, in its order
 template <class E, int D>
-__global__ __launch_bounds__(256) void window_sink_kernel(const float* part, int slots, int bks, int S, int Tk,
-                                                          uint16_t* dk, uint16_t* dv, float scale) {
+__global__ __launch_bounds__(256) void window_sum_kernel(const float* part, int parts, int spans, int64_t bks, int rows,
+                                                         int S, int Tk, uint16_t* dk, uint16_t* dv, float scale) {
   constexpr int PER = D / 4;                           // threads of one row of one of dk, dv
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int c = (int)(u % PER) * 4, which = (int)(u / PER) & 1;
   const int64_t row = u / (2 * PER);
-  if (row >= (int64_t)bks * S) return;
-  const int bk = (int)(row / S), j = (int)(row - (int64_t)bk * S);
-  if (j >= Tk) return;
+  if (row >= bks * rows) return;
+  const int64_t bk = row / rows;
+  const int j = (int)(row - bk * rows);
+  const float* p = part + which * D + c;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < slots; ++i)
-    v += *(const f32x4*)(part + (((int64_t)i * bks + bk) * S + j) * 2 * D + which * D + c);
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) v += *(const f32x4*)(p + ((i * bks + bk) * rows + j) * 2 * D);
+  if (j < S)
+#pragma unroll 8
+    for (int i = 0; i < 4 * spans; ++i)
+      v += *(const f32x4*)(p + (parts * bks * rows + (i * bks + bk) * S + j) * 2 * D);
   v *= which ? 1.f / (1 << E::kShift) : scale;
-  *(uint2*)((which ? dv : dk) + ((int64_t)bk * Tk + j) * D + c) =
-      make_uint2(E::pack2(v[0], v[1]), E::pack2(v[2], v[3]));
+  *(uint2*)((which ? dv : dk) + (bk * Tk + j) * D + c) = make_uint2(E::pack2(v[0], v[1]), E::pack2(v[2], v[3]));
 }
 
 // ------------------------------------------------------------------------------------ few queries
@@ -928,23 +963,24 @@ int fwd(const WinArgs& a, void* o, void* rest, void* lse, hipStream_t st) {
 }
 
 template <class E, int D>
-int bwd(const WinArgs& a, const void* o, const void* rest, const void* dout, const void* lse, void* dsum, void* dq, void* dk,
-        void* dv, void* part, int spans, int span, float scale, hipStream_t st) {
-  const int64_t n = (int64_t)((a.Tq + BM - 1) / BM) * a.B * a.H;
-  const int64_t nk = ((int64_t)(a.Tk + BM - 1) / BM + (int64_t)((a.S + 31) / 32) * spans) *
-                     a.B * a.KV;
+int bwd(const WinArgs& a, const void* o, const void* rest, const void* dout, const void* lse, void* dsum, void* dq,
+        void* dk, void* dv, void* part, int parts, int spans, int span, float scale, hipStream_t st) {
+  const int64_t n = (int64_t)((a.Tq + BM - 1) / BM) * a.B * a.H, bks = (int64_t)a.B * a.KV;
+  const int64_t near = (int64_t)((a.Tk + BM - 1) / BM) * parts * bks;
+  const int64_t nk = near + (((int64_t)((a.S + 31) / 32) * spans * bks + 7) & ~7ll);
   if (n >= (1ll << 31) || nk >= (1ll << 31)) return 1;
   hipLaunchKernelGGL((window_dq_kernel<E, D>), dim3((unsigned)n), dim3(256), 0, st, a, (const uint16_t*)o,
                      (const uint16_t*)rest, (const uint16_t*)dout, (const float*)lse, (float*)dsum, (uint16_t*)dq,
                      scale);
   hipLaunchKernelGGL((window_dkv_kernel<E, D>), dim3((unsigned)nk), dim3(256), 0, st, a, (const uint16_t*)dout,
-                     (const float*)lse, (const float*)dsum, (uint16_t*)dk, (uint16_t*)dv, (float*)part, spans,
+                     (const float*)lse, (const float*)dsum, (uint16_t*)dk, (uint16_t*)dv, (float*)part, parts, spans,
                      span, scale);
-  if (spans) {
-    const int64_t threads = (int64_t)a.B * a.KV * a.S * 2 * (D / 4);
-    if ((threads + 255) / 256 >= (1ll << 31)) return 1;
-    hipLaunchKernelGGL((window_sink_kernel<E, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st,
-                       (const float*)part, 1 + spans, a.B * a.KV, a.S, a.Tk, (uint16_t*)dk, (uint16_t*)dv, scale);
+  if (parts > 1 || spans) {
+    const int rows = parts > 1 ? a.Tk : a.S;
+    const int64_t blocks = (bks * rows * 2 * (D / 4) + 255) / 256;
+    if (blocks >= (1ll << 31)) return 1;
+    hipLaunchKernelGGL((window_sum_kernel<E, D>), dim3((unsigned)blocks), dim3(256), 0, st, (const float*)part, parts,
+                       spans, bks, rows, spans ? a.S : 0, a.Tk, (uint16_t*)dk, (uint16_t*)dv, scale);
   }
   return (int)hipGetLastError();
 }
@@ -991,21 +1027,23 @@ int mopt_window_step(const void* q, const void* k, const void* v, const int64_t*
 }
 
 // dq [B][H][Tq][D], dk, dv [B][KV][Tk][D]; dsum: floats of workspace; part: workspace of
-// (1 + spans) B KV S 2 D floats, spans * span >= Tq (spans 0: no sink is seen out of its window);
+// (parts R + 4 spans S) B KV 2 D floats, R = Tk where parts > 1, else S; parts: shares of each key
+// block's queries; spans * span >= Tq (spans 0: no sink is seen out of its window);
 // lse, dsum: rows of Tq rounded up to 128
 int mopt_window_bwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* start,
                     const void* lengths, int start0, const void* o, const void* rest, const void* dout, const void* lse, void* dsum,
-                    void* dq, void* dk, void* dv, void* part, int spans, int span, int B, int H, int KV, int Tq,
+                    void* dq, void* dk, void* dv, void* part, int parts, int spans, int span, int B, int H, int KV, int Tq,
                     int Tk, int D, int W, int S, float scale, int dtype, void* stream) {
   const WinArgs a = args(q, k, v, strides, start, lengths, start0, B, H, KV, Tq, Tk, W, S, scale);
-  if (!good(a, D) || spans < 0 || span <= 0 || span % BN || (spans && (!part || S == 0))) return 1;
+  if (!good(a, D) || parts < 1 || spans < 0 || span <= 0 || span % BN) return 1;
+  if ((parts > 1 || spans) && !part || (spans && S == 0)) return 1;
   if (S && Tk > W && (int64_t)spans * span < Tq) return 1;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0)
-    return D == 64 ? bwd<Bf16, 64>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, spans, span, scale, st)
-                   : bwd<Bf16, 128>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, spans, span, scale, st);
-  return D == 64 ? bwd<Fp16, 64>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, spans, span, scale, st)
-                 : bwd<Fp16, 128>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, spans, span, scale, st);
+    return D == 64 ? bwd<Bf16, 64>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, parts, spans, span, scale, st)
+                   : bwd<Bf16, 128>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, parts, spans, span, scale, st);
+  return D == 64 ? bwd<Fp16, 64>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, parts, spans, span, scale, st)
+                 : bwd<Fp16, 128>(a, o, rest, dout, lse, dsum, dq, dk, dv, part, parts, spans, span, scale, st);
 }
 
 }  // extern "C"

@@ -30,7 +30,7 @@ _lib.register_signatures({
                         [c_float, c_int, c_void_p], c_int),
     "mopt_window_step": ([c_void_p] * 6 + [c_int] + [c_void_p] * 2 + [c_int] * 9 +
                          [c_float, c_int, c_void_p], c_int),
-    "mopt_window_bwd": ([c_void_p] * 6 + [c_int] + [c_void_p] * 9 + [c_int] * 10 +
+    "mopt_window_bwd": ([c_void_p] * 6 + [c_int] + [c_void_p] * 9 + [c_int] * 11 +
                         [c_float, c_int, c_void_p], c_int),
 })
 
@@ -308,8 +308,14 @@ def window_attention_ref(q, k, v, window=None, sinks=0, scale=None, start=None, 
     return o.reshape(B, H, Tq, D).permute(0, 2, 1, 3).reshape(B * Tq, H * D).to(q.dtype)
 
 
-#: queries of one out-of-window item of the dK / dV kernel (csrc/lm_window.hip)
-_SINK_SPAN = 512
+def _span(window: int, sinks: int, heads: int, Tq: int) -> int:
+    """Queries of one item of the dK / dV kernel that adds up sinks' pairs out of the window
+    (csrc/lm_window.hip): 512 where these items fill the CUs (125M step: 91 us, with 128 117), else
+    about as many as an item within the window has (a window of 100, 14 key heads: 20 us, with 512
+    31); and so many that the 4 partial sums of the sinks' rows that each leaves are no more than
+    there are queries."""
+    near = 512 if heads * -(-Tq // 512) >= 512 else max(128, min(512, -(-window // 64) * 64))
+    return max(near, -(-4 * sinks // 64) * 64)
 
 
 def _geometry(q, k, v):
@@ -346,6 +352,14 @@ def _window_fwd(q, k, v, window, sinks, scale, start, start0, lengths, train):
     return o, rest, lse
 
 
+def _parts(blocks: int, steps: int, D: int) -> int:
+    """Workgroups that share the queries of each of ``blocks`` key blocks in the dK / dV kernel,
+    where there are fewer blocks than the CUs take at once (two each for heads of 64, 8192 tokens of
+    4 key heads, window 1024: 123 + 9 us against 167; one for heads of 128), each with 8 of the
+    block's ``steps`` groups of 32 queries at least.  Their sums are added up by another launch."""
+    return max(1, min((512 if D == 64 else 256) // max(1, blocks), steps // 8))
+
+
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, scale, start, start0, lengths):
@@ -365,12 +379,16 @@ class _WindowAttention(torch.autograd.Function):
         if not o.numel() or not Tk:
             return (dq.zero_(), dk.zero_(), dv.zero_()) + (None,) * 6
         dsum = torch.empty_like(lse)
-        spans = -(-Tq // _SINK_SPAN) if sinks and Tk > window else 0
-        part = torch.empty((1 + spans) * B * KV * sinks * 2 * D if spans else 0,
-                           dtype=torch.float32, device=q.device)
+        span = _span(window, sinks, B * KV, Tq)
+        spans = -(-Tq // span) if sinks and Tk > window else 0
+        parts = _parts(B * KV * -(-Tk // 128), H // KV * (min(Tq, window + 128) // 32), D)
+        part = None
+        if parts > 1 or spans:
+            rows = parts * (Tk if parts > 1 else sinks) + 4 * spans * sinks
+            part = torch.empty(rows * B * KV * 2 * D, dtype=torch.float32, device=q.device)
         _call(q, "mopt_window_bwd", _p(q), _p(k), _p(v), _geometry(q, k, v), _p(start), _p(lengths),
               start0, _p(o), _p(rest), _p(_dense16(do)), _p(lse), _p(dsum), _p(dq), _p(dk), _p(dv), _p(part),
-              spans, _SINK_SPAN, B, H, KV, Tq, Tk, D, window, sinks, scale, _TYPES[q.dtype])
+              parts, spans, span, B, H, KV, Tq, Tk, D, window, sinks, scale, _TYPES[q.dtype])
         return (dq, dk, dv) + (None,) * 6
 
 
