@@ -46,6 +46,14 @@ _lib.register_signatures({
 })
 
 
+def _tensors(y):
+    return y if isinstance(y, tuple) else (y,)
+
+
+def _shapes(y):
+    return [t.shape for t in _tensors(y)]
+
+
 class FlatPopulation:
     optimizer = "adamw"            # or "sgd"
     moment_dtype = torch.float32   # AdamW first-moment storage (bf16: see lm_ops.hip adamw)
@@ -273,7 +281,8 @@ class FlatPopulation:
         return t.unsqueeze(0).expand(self.capacity, *t.shape).contiguous()
 
     def train_step(self, x: torch.Tensor, y: torch.Tensor) -> None:
-        """One optimizer step of every member on the shared batch (x, y).
+        """One optimizer step of every member on the shared batch (x, y); y is a tensor or, for
+        losses that take more than labels, a tuple of tensors.
 
         On a GPU the whole step -- forward, backward, gradient clipping and the fused optimizer
         -- is captured once into a HIP graph and replayed (the per-step host cost of autograd
@@ -311,17 +320,19 @@ class FlatPopulation:
 
     def _graph_step(self, x, y):
         from ..ops._lib import upload_bytes_into
-        if self._graph is None or self._gx.shape != x.shape or self._gy.shape != y.shape:
+        if self._graph is None or self._gx.shape != x.shape or _shapes(self._gy) != _shapes(y):
             self._capture(x, y)
         self._gx.copy_(x)
-        self._gy.copy_(y)
+        for a, b in zip(_tensors(self._gy), _tensors(y)):
+            a.copy_(b)
         upload_bytes_into(self._hp_dev, self.opt_hp)
         self._graph.replay()
 
     def _capture(self, x, y):
         from ..ops._lib import upload_bytes
         self._gx = x.detach().clone()
-        self._gy = y.detach().clone()
+        self._gy = (tuple(t.detach().clone() for t in y) if isinstance(y, tuple)
+                    else y.detach().clone())
         self._hp_dev = upload_bytes(self.opt_hp, self.device)
         state = [self.master_buf, self.p16, self.m, self.v, self.aux, self.stats]
         backup = [t.clone() for t in state]

@@ -247,6 +247,9 @@ class HypergradLM:
         if seq_len is not None:
             import dataclasses
             cfg = dataclasses.replace(cfg, seq_len=seq_len)
+        if not cfg.plain_attention:
+            raise ValueError("hypergradients are taken of plain causal attention only (no qk_norm, "
+                             "kv_heads or window)")
         self.cfg = cfg
         self.device = torch.device(device)
         self.P = P = int(capacity)

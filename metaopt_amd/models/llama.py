@@ -20,6 +20,12 @@ The member interface (``set_member``, ``update_hparams``, ``save_states``/``load
 ``evaluate_async``, ...) is the one :class:`~metaopt_amd.worker.population_sweep.PopulationSweep`
 drives for the MLP population, so the same sweep runs ASHA / PBT / TPE over LMs.
 
+Options of :class:`LMConfig` (off in the presets): RMS norms of the query and key heads
+(``qk_norm``), fewer key heads than query heads (``kv_heads``), a sliding attention window with sink
+tokens (``window``, ``sinks``) -- :mod:`metaopt_amd.ops.heads`; ``PopulationLM(distill=...)`` trains
+on a teacher's top logits beside the labels (:mod:`metaopt_amd.ops.distill`), and
+:meth:`PopulationLM.greedy` continues prompts over a key / value cache.
+
 Presets: ``llama-125m`` (d 768, 12 layers, 12 heads, SwiGLU 2048, vocab 32000; ~134M params with
 an untied head) and ``tiny-2layer`` (the 2-layer LM of config 4).
 """
@@ -28,12 +34,14 @@ from __future__ import annotations
 import dataclasses
 import math
 from dataclasses import dataclass
-from typing import ClassVar, Dict, Optional
+from typing import ClassVar, Dict, Optional, Tuple
 
 import numpy as np
 import torch
 
+from ..ops import heads
 from ..ops import lm as ops
+from ..ops.distill import distill_loss
 from ..ops.gemm import pbmm
 from ..ops.population import MemberConfig
 from .flatpop import FlatPopulation
@@ -49,10 +57,33 @@ class LMConfig:
     rope_base: float = 10000.0
     norm_eps: float = 1e-5
     init_std: float = 0.02
+    qk_norm: bool = False              # RMS norm, with a weight, of every query and key head
+    kv_heads: Optional[int] = None     # key / value heads (None: n_heads); needs qk_norm
+    window: Optional[int] = None       # tokens a query sees back, itself included (None: all)
+    sinks: int = 0                     # first tokens seen whatever the window
 
     @property
     def head_dim(self) -> int:
         return self.d_model // self.n_heads
+
+    @property
+    def key_heads(self) -> int:
+        return self.n_heads if self.kv_heads is None else self.kv_heads
+
+    @property
+    def plain_attention(self) -> bool:
+        """Causal attention over all tokens without head norms or shared key heads."""
+        return not self.qk_norm and self.key_heads == self.n_heads and self.window is None
+
+    def check_heads(self) -> None:
+        if self.key_heads < 1 or self.n_heads % self.key_heads:
+            raise ValueError(f"{self.n_heads} heads are not a multiple of {self.key_heads} key heads")
+        if self.key_heads != self.n_heads and not self.qk_norm:
+            raise ValueError("kv_heads needs qk_norm")
+        if (self.window is not None and self.window < 1) or self.sinks < 0:
+            raise ValueError(f"window {self.window}, sinks {self.sinks}")
+        if self.sinks and self.window is None:
+            raise ValueError("sinks are seen beyond a window: give one")
 
 
 PRESETS = {
@@ -68,14 +99,17 @@ def param_specs(cfg: LMConfig):
     d, F, V, L = cfg.d_model, cfg.ffn, cfg.vocab, cfg.n_layers
     out_std = cfg.init_std / math.sqrt(2 * L)
     specs = [("embed", (V, d), ("normal", cfg.init_std))]
+    qkv = (cfg.n_heads + 2 * cfg.key_heads) * cfg.head_dim
     for l in range(L):
         specs += [(f"l{l}.attn_norm", (d,), ("ones",)),
-                  (f"l{l}.wqkv", (d, 3 * d), ("normal", cfg.init_std)),
+                  (f"l{l}.wqkv", (d, qkv), ("normal", cfg.init_std)),
                   (f"l{l}.wo", (d, d), ("normal", out_std)),
                   (f"l{l}.mlp_norm", (d,), ("ones",)),
                   (f"l{l}.wgu", (d, 2 * F), ("normal", cfg.init_std)),
                   (f"l{l}.wdown", (F, d), ("normal", out_std))]
     specs += [("final_norm", (d,), ("ones",)), ("head", (d, V), ("normal", cfg.init_std))]
+    if cfg.qk_norm:        # together: one run of the gradient buffer to clear
+        specs += [(f"l{l}.{kind}_norm", (cfg.head_dim,), ("ones",)) for l in range(L) for kind in "qk"]
     return specs
 
 
@@ -95,21 +129,37 @@ class PopulationLM(FlatPopulation):
     def __init__(self, capacity: int, config="tiny-2layer", batch_size: int = 8,
                  seq_len: Optional[int] = None, device="cuda", max_grad_norm: float = 1.0,
                  eval_batch: Optional[int] = None, use_graph: bool = True,
-                 moment_dtype: Optional[torch.dtype] = None):
+                 moment_dtype: Optional[torch.dtype] = None,
+                 distill: Optional[Tuple[float, float]] = None):
+        """``distill``: (alpha, temperature) of :func:`~metaopt_amd.ops.distill.distill_loss` --
+        training batches are then (tokens, (labels, teacher's top logits, their indices)), as
+        ``SyntheticLM(teacher_top=...)`` gives them.  ``self.alpha`` and ``self.temperature`` hold
+        one value a trial and may be written in place between steps."""
         if moment_dtype is not None:       # AdamW first-moment storage (mopt sweep --dtype)
             self.moment_dtype = moment_dtype
         self.cfg = PRESETS[config] if isinstance(config, str) else config
         if seq_len is not None:
             self.cfg = dataclasses.replace(self.cfg, seq_len=seq_len)
         c = self.cfg
-        if c.head_dim != 64 or c.seq_len % 64:
-            raise ValueError("the attention kernel needs head_dim 64 and seq_len % 64 == 0")
+        c.check_heads()
+        if c.head_dim not in ((64, 128) if c.qk_norm else (64,)) or c.seq_len % 64:
+            raise ValueError("the attention kernel needs head_dim 64 (128 too with qk_norm) and "
+                             "seq_len % 64 == 0")
         self.batch_size = int(batch_size)          # sequences per trial per step
         self.eval_batch = int(eval_batch or batch_size)
         self.tokens_per_step = self.batch_size * c.seq_len
         super().__init__(capacity, device=device, max_grad_norm=max_grad_norm,
                          use_graph=use_graph)
-        self.cos, self.sin = ops.rope_tables(c.seq_len, c.rope_base, device=self.device)
+        self.cos, self.sin = (ops.rope_tables(c.seq_len, c.rope_base, device=self.device)
+                              if not c.qk_norm else
+                              heads.rope_tables(c.seq_len, c.head_dim, c.rope_base, self.device))
+        self.distill = distill is not None
+        if self.distill:
+            alpha, temperature = (float(x) for x in distill)
+            if not (0.0 <= alpha <= 1.0 and temperature > 0.0):
+                raise ValueError(f"distill {distill}: (alpha in [0, 1], temperature > 0)")
+            full = lambda x: torch.full((self.capacity,), x, device=self.device)  # noqa: E731
+            self.alpha, self.temperature = full(alpha), full(temperature)
 
     def param_specs(self):
         return param_specs(self.cfg)
@@ -118,8 +168,9 @@ class PopulationLM(FlatPopulation):
     moment_dtype = torch.bfloat16
 
     def direct_grads(self):
-        # projections (pgemm grad_out), norms and the embedding (cast into the .grad views)
-        return {name for name, _, _ in self.specs}
+        # projections (pgemm grad_out), norms and the embedding (cast into the .grad views); the
+        # head norms' gradients are added by autograd
+        return {name for name, _, _ in self.specs if not name.endswith((".q_norm", ".k_norm"))}
 
     def rows_per_batch(self, x) -> int:
         return int(x.numel())
@@ -127,22 +178,37 @@ class PopulationLM(FlatPopulation):
     def train_rows(self) -> int:
         return self.tokens_per_step
 
-    def _loss(self, tok: torch.Tensor, labels: torch.Tensor, train: bool):
+    def _loss(self, tok: torch.Tensor, labels, train: bool):
+        top = None
+        if isinstance(labels, tuple):
+            labels, *top = labels
         tok, labels = self._expand(tok, torch.int32), self._expand(labels, torch.int32)
-        c, P = self.cfg, self.capacity
-        T, d, H = c.seq_len, c.d_model, c.n_heads
-        rpt = tok.numel() // P
-        R = tok.numel()
-        W = self.W
+        P, rpt, V = self.capacity, tok.numel() // self.capacity, self.cfg.vocab
+        logits = self._logits(tok.view(P, -1, self.cfg.seq_len), self._attention)
+        labels = labels.reshape(-1)
+        if not train:
+            return ops.ce_eval(logits, labels, rpt)
+        if not self.distill:
+            return ops.cross_entropy(logits, labels, rpt, grad_scale=1.0 / rpt, unit_weights=True)
+        if top is None:
+            raise ValueError("distillation takes batches (tokens, (labels, top values, top indices))")
+        values, index = (self._expand(t, kind).reshape(P * rpt, -1)
+                         for t, kind in zip(top, (None, torch.int32)))
+        return distill_loss(logits, labels, values, index, rpt, self.temperature, self.alpha,
+                            grad_scale=1.0 / rpt, unit_weights=True, inplace=True)
+
+    def _logits(self, tok: torch.Tensor, attend):
+        """Rows of logits of the tokens ``[P, sequences, T]``; ``attend(l, h, T)``: layer l's
+        attention output of the normalised rows h."""
+        c, P, W = self.cfg, self.capacity, self.W
+        R, T, d = tok.numel(), tok.shape[-1], c.d_model
+        rpt = R // P
         x = ops.embedding(tok.reshape(-1), W["embed"], rpt)
         # every residual add is fused into the pre-norm that follows it (ops.add_rmsnorm); the
         # embedding's two gradients (residual stream, first norm) meet in that norm's backward
         x, h = ops.rmsnorm_pass(x, W["l0.attn_norm"], rpt, c.norm_eps)
         for l in range(c.n_layers):
-            # interleaved-pair RoPE applied by the QKV GEMM's epilogue and, backward, by the
-            # attention kernels' gradient outputs (ops.qkv_rope_attention)
-            o = ops.qkv_rope_attention(h.view(P, rpt, d), W[f"l{l}.wqkv"], self.cos, self.sin,
-                                       T, H)
+            o = attend(l, h.view(P, rpt, d), T)
             x, h = ops.add_rmsnorm(x, _lin(o.view(P, rpt, d), W[f"l{l}.wo"]).view(R, d),
                                    W[f"l{l}.mlp_norm"], rpt, c.norm_eps)
             # gate / up columns interleaved in 16-column groups: the SwiGLU runs in the GEMM
@@ -150,20 +216,65 @@ class PopulationLM(FlatPopulation):
             y = ops.swiglu_mlp(h.view(P, rpt, d), W[f"l{l}.wgu"], W[f"l{l}.wdown"])
             nxt = W[f"l{l + 1}.attn_norm"] if l + 1 < c.n_layers else W["final_norm"]
             x, h = ops.add_rmsnorm(x, y.view(R, d), nxt, rpt, c.norm_eps)
-        logits = _lin(h.view(P, rpt, d), W["head"]).view(R, c.vocab)
-        if train:
-            return ops.cross_entropy(logits, labels.reshape(-1), rpt, grad_scale=1.0 / rpt,
-                                     unit_weights=True)
-        return ops.ce_eval(logits, labels.reshape(-1), rpt)
+        return _lin(h.view(P, rpt, d), W["head"]).view(R, c.vocab)
+
+    def _attention(self, l, h, T):
+        c, W = self.cfg, self.W
+        if c.plain_attention:
+            # interleaved-pair RoPE applied by the QKV GEMM's epilogue and, backward, by the
+            # attention kernels' gradient outputs (ops.qkv_rope_attention)
+            return ops.qkv_rope_attention(h, W[f"l{l}.wqkv"], self.cos, self.sin, T, c.n_heads)
+        if c.qk_norm:
+            qkv = _lin(h, W[f"l{l}.wqkv"]).flatten(0, 1)
+            q, k, v = heads.qk_norm_rope(qkv, W[f"l{l}.q_norm"], W[f"l{l}.k_norm"], self.cos, self.sin,
+                                         T, c.n_heads, c.key_heads, c.norm_eps, il=True)
+        else:
+            q, k, v = ops.qkv_rope(h, W[f"l{l}.wqkv"], self.cos, self.sin, T, c.n_heads)
+        return heads.window_attention(q, k, v, c.window, c.sinks)
+
+    @torch.no_grad()
+    def greedy(self, tok: torch.Tensor, steps: int) -> torch.Tensor:
+        """The ``steps`` most likely next tokens, one after another, ``[P, sequences, steps]`` of
+        every trial for the prompts ``tok`` ``[sequences, T]``, over a cache of keys and values
+        (``qk_norm`` models; ``T + steps <= seq_len + 1``)."""
+        c, P, W = self.cfg, self.capacity, self.W
+        n, T = tok.shape
+        if not c.qk_norm:
+            raise ValueError("continuations need a model with qk_norm")
+        if T < 1 or steps < 1 or T + steps > c.seq_len + 1:
+            raise ValueError(f"{T} + {steps} tokens: a prompt and a step at least, and at most "
+                             f"{c.seq_len + 1}")
+        shape = (c.n_layers, P * n, c.key_heads, T + steps - 1, c.head_dim)
+        kcache, vcache = (torch.zeros(shape, dtype=W["embed"].dtype, device=self.device)
+                          for _ in "kv")
+        start = torch.zeros(P * n, dtype=torch.int32, device=self.device)
+
+        def attend(l, h, T):
+            qkv = _lin(h, W[f"l{l}.wqkv"]).flatten(0, 1)
+            q = heads.qk_norm_rope_cached(qkv, W[f"l{l}.q_norm"], W[f"l{l}.k_norm"], self.cos, self.sin,
+                                          T, c.n_heads, kcache[l], vcache[l], start, c.norm_eps, il=True)
+            return heads.window_attention(q, kcache[l], vcache[l], c.window, c.sinks, start=start)
+        out, tok = [], self._expand(tok, torch.int32)
+        for _ in range(steps):
+            logits = self._logits(tok, attend).view(P, n, -1, c.vocab)
+            start += tok.shape[-1]
+            tok = logits[:, :, -1:].argmax(-1).to(torch.int32)
+            out.append(tok)
+        return torch.cat(out, -1)
 
 
 class SyntheticLM:
     """Token streams from a fixed random sparse bigram model (so the loss can fall well below
     ``log(vocab)``): every token has ``branch`` likely successors.  Pre-generated on the host
-    with numpy (vectorised over many chains), stored on the device, sliced per step."""
+    with numpy (vectorised over many chains), stored on the device, sliced per step.
+
+    ``teacher_top``: training batches are (tokens, (labels, values, indices)) with the model's own
+    largest log-probabilities of each next token, that many or ``branch`` of them (a successor may
+    come twice), for ``PopulationLM(distill=...)``."""
 
     def __init__(self, vocab: int, seq_len: int, batch_size: int, n_tokens: int = 1 << 21,
-                 branch: int = 8, seed: int = 0, device=None, n_val_seq: Optional[int] = None):
+                 branch: int = 8, seed: int = 0, device=None, n_val_seq: Optional[int] = None,
+                 teacher_top: int = 0):
         rng = np.random.default_rng(seed)
         self.vocab, self.seq_len, self.batch_size = vocab, seq_len, batch_size
         succ = rng.integers(0, vocab, size=(vocab, branch))
@@ -183,10 +294,19 @@ class SyntheticLM:
         self.train = torch.from_numpy(toks[n_val:]).to(dev)
         self.val = torch.from_numpy(toks[:n_val]).to(dev)
         self.n_batches = len(self.train) // batch_size
+        self.top = None
+        if teacher_top:
+            order = np.argsort(-probs, 1, kind="stable")[:, :teacher_top]
+            with np.errstate(divide="ignore"):
+                values = np.log(np.take_along_axis(probs, order, 1)).astype(np.float32)
+            index = np.take_along_axis(succ, order, 1).astype(np.int32)
+            self.top = torch.from_numpy(values).to(dev), torch.from_numpy(index).to(dev)
 
     def batch(self, step: int):
         i = step % self.n_batches
         b = self.train[i * self.batch_size:(i + 1) * self.batch_size]
+        if self.top is not None:
+            return b[:, :-1], (b[:, 1:], *(t[b[:, :-1].long()] for t in self.top))
         return b[:, :-1], b[:, 1:]
 
     def validation(self):

@@ -121,16 +121,20 @@ def _resnet(population, device, seed, batch_size=128, blocks=3, image_size=32, p
 
 
 def _lm(population, device, seed, preset="llama-125m", batch_size=8, seq_len=512, priors=None,
-        state_dtype="bf16", **kw):
+        state_dtype="bf16", model=None, distill=None, teacher_top=8, **kw):
+    """``model``: LMConfig fields that differ from the preset's (qk_norm, kv_heads, window, sinks);
+    ``distill``: (alpha, temperature), with the data's own ``teacher_top`` logits as the teacher."""
+    import dataclasses
     import torch
     from ..models.llama import PRESETS, LM_PBT_PRIORS, LMSweepTask, PopulationLM, SyntheticLM
-    cfg = PRESETS[preset]
+    cfg = dataclasses.replace(PRESETS[preset], **(model or {}))
     task = LMSweepTask(priors=dict(priors or LM_PBT_PRIORS), d_model=cfg.d_model)
-    pop = PopulationLM(population, preset, batch_size=batch_size, seq_len=seq_len,
+    pop = PopulationLM(population, cfg, batch_size=batch_size, seq_len=seq_len, distill=distill,
                        device=device, moment_dtype=(torch.bfloat16 if state_dtype == "bf16"
                                                     else torch.float32))
     data = SyntheticLM(cfg.vocab, seq_len, batch_size, n_tokens=kw.get("n_tokens", 1 << 22),
-                       seed=seed, device=device)
+                       seed=seed, device=device,
+                       teacher_top=teacher_top if distill is not None else 0)
     return task, pop, data
 
 
