@@ -152,18 +152,32 @@ __device__ __forceinline__ void wait_barrier() {
 template <int D, int ROWS = BN>
 constexpr int kFills = ROWS * D * 2 / 1024 / 4;        // 1 KB fills of a tile by each of 4 waves
 
+// A tile of rows row0 ... of a matrix.  Where each lane reads is kept for the tiles whose rows all lie
+// inside [lo, hi): with the rows clamped one by one for every tile a fill was 25 vector instructions.
 template <int D, int ROWS = BN>
-__device__ __forceinline__ void fill_tile(const uint16_t* g, int64_t ld, int row0, int lo, int hi, uint16_t* img,
-                                          int wave, int lane) {
-  constexpr int CH = D / 8, PER = 64 / CH;             // chunks of a row, rows of a fill
-  const char* base = scalar(g + row0 * ld);
-  const int first = lo - row0, last = hi - 1 - row0;   // (last >= 0: a tile starts inside)
+struct Fill {
+  static constexpr int N = kFills<D, ROWS>, CH = D / 8, PER = 64 / CH;   // chunks of a row, rows of a fill
+  uint32_t off[N], row;                                // bytes from row0's start and of a row
+  int wave, lane;
+  __device__ __forceinline__ Fill(int64_t ld, int wave, int lane) : row((uint32_t)ld * 2), wave(wave), lane(lane) {
 #pragma unroll
-  for (int j = 0; j < kFills<D, ROWS>; ++j) {
-    const int blk = wave * kFills<D, ROWS> + j, r = blk * PER + lane / CH, c = (lane % CH) ^ swz<D>(r);
-    fill16(base, (uint32_t)max(first, min(last, r)) * ((uint32_t)ld * 2) + c * 16, img + blk * 512);
+    for (int j = 0; j < N; ++j) off[j] = r(j) * row + c(j) * 16;
   }
-}
+  __device__ __forceinline__ int r(int j) const { return (wave * N + j) * PER + lane / CH; }
+  __device__ __forceinline__ int c(int j) const { return (lane % CH) ^ swz<D>(r(j)); }
+  __device__ __forceinline__ void tile(const uint16_t* g, int row0, int lo, int hi, uint16_t* img) const {
+    const char* base = scalar((const char*)g + (int64_t)row0 * row);
+    const int first = lo - row0, last = hi - 1 - row0;   // (last >= 0: a tile starts inside)
+    if (first <= 0 && last >= ROWS - 1) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) fill16(base, off[j], img + (wave * N + j) * 512);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        fill16(base, (uint32_t)max(first, min(last, r(j))) * row + c(j) * 16, img + (wave * N + j) * 512);
+    }
+  }
+};
 
 // waves a SIMD (registers: 512 / waves) and ring of a kernel (tiles of two matrices)
 template <int D> constexpr int kDkvWaves = D == 64 ? 3 : 2;
@@ -302,9 +316,10 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
     const uint16_t* vg = a.v + b * a.v_sb + hk * a.v_sh;
     const Tiles tiles(s.st + bt0, s.st + bt1, a.W, a.S);
     // (slot of tile 0: 1)
+    const Fill<D> kfill(a.k_st, wave, lane), vfill(a.v_st, wave, lane);
     auto fetch = [&](int it) {
-      fill_tile<D>(kg, a.k_st, tiles.key(it), 0, s.len, ring[(it + 1) % NS][0], wave, lane);
-      fill_tile<D>(vg, a.v_st, tiles.key(it), 0, s.len, ring[(it + 1) % NS][1], wave, lane);
+      kfill.tile(kg, tiles.key(it), 0, s.len, ring[(it + 1) % NS][0]);
+      vfill.tile(vg, tiles.key(it), 0, s.len, ring[(it + 1) % NS][1]);
     };
     Rows<D>::fill(a.q + b * a.q_sb + hq * a.q_sh, a.q_st, tw, s.t0, s.t1, img, lane);
     for (int it = 0; it < min(NS - 1, tiles.n); ++it) fetch(it);
@@ -414,9 +429,10 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
     const uint16_t* kg = a.k + b * a.k_sb + hk * a.k_sh;
     const uint16_t* vg = a.v + b * a.v_sb + hk * a.v_sh;
     const Tiles tiles(s.st + bt0, s.st + bt1, a.W, a.S);
+    const Fill<D> kfill(a.k_st, wave, lane), vfill(a.v_st, wave, lane);
     auto fetch = [&](int it) {
-      fill_tile<D>(kg, a.k_st, tiles.key(it), 0, s.len, ring[(it + 1) % NS][0], wave, lane);
-      fill_tile<D>(vg, a.v_st, tiles.key(it), 0, s.len, ring[(it + 1) % NS][1], wave, lane);
+      kfill.tile(kg, tiles.key(it), 0, s.len, ring[(it + 1) % NS][0]);
+      vfill.tile(vg, tiles.key(it), 0, s.len, ring[(it + 1) % NS][1]);
     };
     Rows<D>::fill(a.q + b * a.q_sb + hq * a.q_sh, a.q_st, tw, s.t0, s.t1, img, lane);
     const float ls = lse[(int64_t)bh * nqb * BM + t];
@@ -523,6 +539,7 @@ struct Dkv {
   const Seq& s;
   int b, hk, tq_pad, lane, wave;
   Place<D> at;
+  Fill<D, QN> qfill, ofill;
   u32x4 kf[DK], vf[kValuesInLds ? 1 : DK];
   f32x16 ak[DN], av[DN];
 
@@ -539,8 +556,8 @@ struct Dkv {
   int row_n, slot_n;
 
   __device__ __forceinline__ void fetch(int tb, int te) {
-    fill_tile<D, QN>(qn, a.q_st, row_n, s.t0, s.t1, lds.ring[slot_n][0], wave, lane);
-    fill_tile<D, QN>(on, (int64_t)a.H * D, row_n, s.t0, s.t1, lds.ring[slot_n][1], wave, lane);
+    qfill.tile(qn, row_n, s.t0, s.t1, lds.ring[slot_n][0]);
+    ofill.tile(on, row_n, s.t0, s.t1, lds.ring[slot_n][1]);
     // (waves 2 and 3 write what waves 0 and 1 do: each has the same number of loads under way)
     fill4(scalar(sn + row_n), 4 * (lane & (QN - 1)), lds.stat[slot_n][wave & 1]);
     slot_n = slot_n + 1 == NS ? 0 : slot_n + 1;
@@ -690,7 +707,8 @@ __global__ __launch_bounds__(256, kDkvWaves<D>) void window_dkv_kernel(
   const int bk = item / (far ? nfar : nkb), it0 = item - bk * (far ? nfar : nkb), b = bk / a.KV, hk = bk - b * a.KV;
   const Seq s = seq_of(a, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  K k{a, dout, lse, dsum, lds, s, b, hk, (a.Tq + BM - 1) / BM * BM, lane, wave, Place<D>(lane)};
+  K k{a, dout, lse, dsum, lds, s, b, hk, (a.Tq + BM - 1) / BM * BM, lane, wave, Place<D>(lane),
+      Fill<D, K::QN>(a.q_st, wave, lane), Fill<D, K::QN>((int64_t)a.H * D, wave, lane)};
   const int G = a.H / a.KV, c = it0 % (far ? spans : parts);
   const int kb = it0 / parts, kw = far ? it0 / spans * 32 : kb * BM + wave * 32;
   const int j = kw + (lane & 31);
