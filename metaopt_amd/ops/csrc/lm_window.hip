@@ -286,6 +286,11 @@ __device__ __forceinline__ void hide(f32x16& x, float with, int i, int k0, int l
   }
 }
 
+// Forward: one pass over the keys with a running reference and sum.  Heads of 64 (4 sequences of 12
+// heads, 4096 tokens, window 512: 51 us, 475 TFLOP/s) are bound by the vector work on the scores, on a
+// SIMD about 670 clocks a group of 32 x 32 pairs beside 256 of products; heads of 128 (8192 tokens of
+// 16 / 4 heads, window 1024: 101 us, 640 TFLOP/s) by LDS: 16 KB of fragments a group and wave, and a
+// third wave a SIMD (tiles of 32 keys) changes nothing.
 template <class E, int D>
 __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a, uint16_t* o, uint16_t* rest,
                                                                        float* lse) {
@@ -398,7 +403,8 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
 // dQ, and D of its rows for the dK / dV kernel.  D is formed from o and what o's rounding left off
 // (`rest`, written by the forward): with o alone its error adds to that of the rounded dS, and where
 // few keys are seen it is the larger one (a window of 4: 1.8 times the error of a once rounded dq
-// instead of 1.5).
+// instead of 1.5).  125M step (64 x 12 heads, 512 tokens, window 128): 84 us, of which reading and
+// writing 350 MB is 65; heads of 128, 8192 tokens, window 1024: 137 us (705 TFLOP/s), LDS-bound as above.
 template <class E, int D>
 __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, const uint16_t* o,
                                                                      const uint16_t* rest, const uint16_t* dout,
@@ -517,9 +523,11 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
 // turns at the groups of 32 queries.
 // What is not a key's whole sum is left in 32 bits: the near sums of all rows (parts > 1) or of rows
 // j < S, [part][b, hk][rows][2][D], and the far ones behind them, [span][wave][b, hk][S][2][D];
-// window_sum_kernel adds them.  Bound by the vector work on the scores (exp2, dS, packing) between the
-// products: 125M step (64 x 12 heads, 512 tokens, window 128, 4 sinks) 90 - 104 us.  (Two waves for each
-// key, 8 a workgroup, were slower everywhere: 272 us.)
+// window_sum_kernel adds them.  125M step (64 x 12 heads, 512 tokens, window 128, 4 sinks): 94 us, bound
+// by the vector work on the scores (exp2, dS, packing) between the products; heads of 128, 8192 tokens,
+// window 1024: 225 us (570 TFLOP/s), bound by LDS: 40 KB of fragments a group of 32 x 32 pairs and wave,
+// the same time with one and two waves a SIMD.  (Two waves for each key, 8 a workgroup, were slower
+// everywhere: 125M step 272 us.)
 template <class E, int D>
 struct Dkv {
   // heads of 128: 64 registers of key and value fragments beside 128 of sums leave too few for the
@@ -771,7 +779,8 @@ __global__ __launch_bounds__(256) void window_sum_kernel(const float* part, int 
 // that go through the keys 32 at a time on their own -- keys from memory into registers as operands,
 // values into LDS for the transposing read, both a chunk ahead -- and join their maxima, sums and
 // products in the end.  With `splits` > 1 the keys of a head are shared among that many workgroups,
-// which leave theirs in `part`, and window_join_kernel joins them.
+// which leave theirs in `part`, and window_join_kernel joins them.  32768 keys of 8 heads of 128: 25.5 us
+// (5.3 TB/s) and 4 for joining.
 // Products are 16x16x32: lane l holds A[l & 15][8 (l >> 4) ..], B[8 (l >> 4) ..][l & 15] and
 // C[4 (l >> 4) + r][l & 15]; the keys of the two score tiles of a chunk are fed so that a lane's
 // 4 + 4 scores are those of keys 8 (l >> 4) ... + 7, the B operand of the product with V.
