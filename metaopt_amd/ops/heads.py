@@ -247,6 +247,9 @@ def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=
         raise ValueError(f"the caches are {tuple(kcache.shape)}: {n} sequences of heads of {D}")
     if kcache.dtype != qkv.dtype or vcache.dtype != qkv.dtype:
         raise ValueError("the caches must be of qkv's type")
+    if any(s == 0 and m > 1 for c in (kcache, vcache) for s, m in zip(c.stride(), c.shape)) or \
+            (kcache.numel() and kcache.data_ptr() == vcache.data_ptr()):
+        raise ValueError("the caches are written: no expanded tensors, and not one for both")
     _same(qkv, "kcache vcache start", kcache, vcache, start)
     _int32("start", start, n)
     if not _hip(qkv, "qk_norm_rope"):

@@ -226,7 +226,9 @@ def test_qk_norm_rope_refuses(bad, match):
     (dict(start=torch.zeros(2)), "int32"), (dict(start=torch.zeros(3, dtype=torch.int32)), "int32"),
     (dict(kcache=torch.zeros(2, 2, 4, 8), vcache=torch.zeros(2, 2, 5, 8)), "alike"),
     (dict(kcache=torch.zeros(3, 2, 4, 8), vcache=torch.zeros(3, 2, 4, 8)), "sequences"),
-    (dict(kcache=torch.zeros(2, 2, 4, 8).half(), vcache=torch.zeros(2, 2, 4, 8).half()), "type")])
+    (dict(kcache=torch.zeros(2, 2, 4, 8).half(), vcache=torch.zeros(2, 2, 4, 8).half()), "type"),
+    (dict(kcache=torch.zeros(1, 2, 4, 8).expand(2, 2, 4, 8)), "written"),
+    (dict(zip(("kcache", "vcache"), [torch.zeros(2, 2, 4, 8)] * 2)), "written")])
 def test_qk_norm_rope_cached_refuses(bad, match):
     d = _qk_args(qkv=torch.zeros(4, 48), kcache=torch.zeros(2, 2, 4, 8), vcache=torch.zeros(2, 2, 4, 8),
                  start=torch.zeros(2, dtype=torch.int32))
