@@ -840,6 +840,9 @@ __global__ __launch_bounds__(NW * 64) void window_step_kernel(WinArgs a, uint16_
     if (c < end) fetch(c, 0);
     for (; c < end; c += NW, buf ^= 1) {
       const int k0 = key(c);
+      // (the keys were loaded behind the values: with one of them here, so are the values, and no
+      // read of theirs comes before this)
+      asm volatile("" : "+v"(kf[0][0]) : : "memory");
       f32x4 x[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -847,7 +850,6 @@ __global__ __launch_bounds__(NW * 64) void window_step_kernel(WinArgs a, uint16_
 #pragma unroll
         for (int ks = 0; ks < DK; ++ks) x[h] = E::mfma16(kf[h][ks], qf[ks], x[h]);
       }
-      // (the keys, loaded behind them, are here: so are the values)
       if (c + NW < end) fetch(c + NW, buf ^ 1);
       float mx = -INFINITY;
 #pragma unroll

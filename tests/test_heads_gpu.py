@@ -359,6 +359,9 @@ def test_offsets_past_32_bits():
     cos, sin = heads.rope_tables(2, D, device=DEV)
     big = (torch.cat([cos] * 1)[:1].expand(Tk, -1).contiguous(), sin[:1].expand(Tk, -1).contiguous())
     kc = heads.qk_norm_rope(x, w, w, cos, sin, 1, 2, 1)
-    heads.qk_norm_rope_cached(x, w, w, *big, 1, 2, k, k,
+    v = torch.zeros_like(k)
+    heads.qk_norm_rope_cached(x, w, w, *big, 1, 2, k, v,
                               torch.full((n,), Tk - 1, device=DEV, dtype=torch.int32))
-    assert torch.equal(k[:, :, Tk - 1], kc[2][:, :, 0])          # the values are written last or first
+    assert torch.equal(v[:, :, Tk - 1], kc[2][:, :, 0])
+    assert torch.equal(k[:, :, Tk - 1], kc[1][:, :, 0])          # (the angle of every row is 0)
+    assert not v[:, :, :Tk - 1].any()
