@@ -515,6 +515,16 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
   if (lane < 32) dsum[(int64_t)bh * nqb * BM + t] = valid ? ds : 0.f;
 }
 
+// v in three bf16 pieces (24 bits), as the row of an A operand that holds them in its first columns and
+// zeros behind; lanes l >= 32, later columns, all zeros
+__device__ __forceinline__ u32x4 pieces(float v, int lane) {
+  v = lane < 32 ? fminf(fmaxf(v, -3e38f), 3e38f) : 0.f;
+  const uint32_t a = Bf16::pack2(v, 0.f);
+  const float v1 = v - Bf16::up(a);
+  const uint32_t b = Bf16::pack2(v1, 0.f);
+  return u32x4{a | b << 16, Bf16::pack2(v1 - Bf16::up(b), 0.f), 0, 0};
+}
+
 // dK, dV.  Two kinds of items:
 // near: 128 keys, 32 a wave, with the queries that have them in their window, or one of `parts` shares
 // of these;
@@ -545,6 +555,7 @@ struct Dkv {
   const float *lse, *dsum;
   Lds& lds;
   const Seq& s;
+  float rc;                                            // 1 / c
   int b, hk, tq_pad, lane, wave;
   Place<D> at;
   Fill<D, QN> qfill, ofill;
@@ -631,17 +642,16 @@ struct Dkv {
   // this lane's key, pairs with values of [0, mine) count (all: every pair does)
   __device__ __forceinline__ void step(int slot, int sub, bool all, int d0, uint32_t mine) {
     const uint32_t Qs = lds_at(lds.ring[slot][0]) + sub * 64 * D, Os = lds_at(lds.ring[slot][1]) + sub * 64 * D;
-    const float *ls = lds.stat[slot][0], *ds = lds.stat[slot][1];
-    f32x16 x = zero16(), y = zero16();
+    // Both products start at what their rows' sums take off: a value of each row in three pieces, times
+    // ones.  (From LDS to the registers that need them the 2 x 16 values would be 8 reads of 1 KB.)
+    const int own = 32 * sub + swap23(lane & 31);
+    const u32x4 ones = {0x3F803F80, 0x3F803F80, 0x3F803F80, 0x3F803F80};
+    f32x16 x = Bf16::mfma32(pieces(-lds.stat[slot][0][own] * rc, lane), ones, zero16());
+    f32x16 y = Bf16::mfma32(pieces(-lds.stat[slot][1][own], lane), ones, zero16());
 #pragma unroll
     for (int ks = 0; ks < DK; ++ks) x = E::mfma32(at.frag(Qs, 0, ks), kf[ks], x);
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const f32x4 l4 = *(const f32x4*)(ls + 32 * sub + row_of(4 * r4, lane));
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        x[4 * r4 + e] = __builtin_amdgcn_exp2f(fmaf(x[4 * r4 + e], a.c, (float)E::kShift - l4[e]));
-    }
+    for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(E::kShift ? fmaf(x[r], a.c, (float)E::kShift) : x[r] * a.c);
     if (!all) {
       const int d = d0 + 8 * (lane >> 5);
 #pragma unroll
@@ -665,13 +675,7 @@ struct Dkv {
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const f32x4 d4 = *(const f32x4*)(ds + 32 * sub + row_of(4 * r4, lane));
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        y[4 * r4 + e] = x[4 * r4 + e] * (E::kShift ? fmaf(d4[e], -kUnshift, y[4 * r4 + e] * kUnshift)
-                                                   : y[4 * r4 + e] - d4[e]);
-    }
+    for (int r = 0; r < 16; ++r) y[r] *= E::kShift ? x[r] * kUnshift : x[r];
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const u32x4 p = pack<E>(x, st);
@@ -715,7 +719,7 @@ __global__ __launch_bounds__(256, kDkvWaves<D>) void window_dkv_kernel(
   const int bk = item / (far ? nfar : nkb), it0 = item - bk * (far ? nfar : nkb), b = bk / a.KV, hk = bk - b * a.KV;
   const Seq s = seq_of(a, b);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  K k{a, dout, lse, dsum, lds, s, b, hk, (a.Tq + BM - 1) / BM * BM, lane, wave, Place<D>(lane),
+  K k{a, dout, lse, dsum, lds, s, 1.f / a.c, b, hk, (a.Tq + BM - 1) / BM * BM, lane, wave, Place<D>(lane),
       Fill<D, K::QN>(a.q_st, wave, lane), Fill<D, K::QN>((int64_t)a.H * D, wave, lane)};
   const int G = a.H / a.KV, c = it0 % (far ? spans : parts);
   const int kb = it0 / parts, kw = far ? it0 / spans * 32 : kb * BM + wave * 32;
