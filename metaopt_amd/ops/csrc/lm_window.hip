@@ -754,27 +754,39 @@ __global__ __launch_bounds__(256, kDkvWaves<D>) void window_dkv_kernel(
   if (some && j < a.Tk) k.put_part(part + ((c * bks + bk) * rows + j) * 2 * D);
 }
 
-// dk, dv of the first `rows` rows of each key head, from what window_dkv_kernel left, in its order
+// dk, dv of the first `rows` rows of each key head, from what window_dkv_kernel left.  Each of the first
+// `wide` rows (the sinks, where they have many sums) takes a workgroup that adds them in slices (256 sums
+// of 4 rows: 14 us with the others, one after another 23; 4 sums of 70 rows of 768 heads: 67, so 31), each
+// 4 columns of the other rows a thread.
 template <class E, int D>
 __global__ __launch_bounds__(256) void window_sum_kernel(const float* part, int parts, int spans, int64_t bks, int rows,
-                                                         int S, int Tk, uint16_t* dk, uint16_t* dv, float scale) {
-  constexpr int PER = D / 4;                           // threads of one row of one of dk, dv
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int c = (int)(u % PER) * 4, which = (int)(u / PER) & 1;
-  const int64_t row = u / (2 * PER);
-  if (row >= bks * rows) return;
-  const int64_t bk = row / rows;
-  const int j = (int)(row - bk * rows);
-  const float* p = part + which * D + c;
+                                                         int S, int wide, int Tk, uint16_t* dk, uint16_t* dv,
+                                                         float scale) {
+  constexpr int PER = 2 * D / 4, SL = 256 / PER;       // threads of a row of both, slices of a workgroup
+  __shared__ f32x4 slices[SL][PER];
+  const int c = threadIdx.x % PER, sl = threadIdx.x / PER, which = c / (PER / 2), col = c % (PER / 2) * 4;
+  const bool slice = blockIdx.x < bks * wide;
+  const int64_t u = slice ? blockIdx.x : (blockIdx.x - bks * wide) * SL + sl;
+  const int per = slice ? wide : rows - wide, first = slice ? sl : 0, by = slice ? SL : 1;
+  if (u >= bks * per) return;                          // (never of a slice)
+  const int64_t bk = u / per;
+  const int j = (int)(u - bk * per) + (slice ? 0 : wide);
+  const float* p = part + c * 4;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = 0; i < parts; ++i) v += *(const f32x4*)(p + ((i * bks + bk) * rows + j) * 2 * D);
+  for (int i = first; i < parts; i += by) v += *(const f32x4*)(p + ((i * bks + bk) * rows + j) * 2 * D);
   if (j < S)
 #pragma unroll 8
-    for (int i = 0; i < 4 * spans; ++i)
+    for (int i = first; i < 4 * spans; i += by)
       v += *(const f32x4*)(p + (parts * bks * rows + (i * bks + bk) * S + j) * 2 * D);
+  if (slice) {
+    slices[sl][c] = v;
+    __syncthreads();
+    if (sl) return;
+    for (int i = 1; i < SL; ++i) v += slices[i][c];
+  }
   v *= which ? 1.f / (1 << E::kShift) : scale;
-  *(uint2*)((which ? dv : dk) + (bk * Tk + j) * D + c) = make_uint2(E::pack2(v[0], v[1]), E::pack2(v[2], v[3]));
+  *(uint2*)((which ? dv : dk) + (bk * Tk + j) * D + col) = make_uint2(E::pack2(v[0], v[1]), E::pack2(v[2], v[3]));
 }
 
 // ------------------------------------------------------------------------------------ few queries
@@ -1009,11 +1021,11 @@ int bwd(const WinArgs& a, const void* o, const void* rest, const void* dout, con
                      (const float*)lse, (const float*)dsum, (uint16_t*)dk, (uint16_t*)dv, (float*)part, parts, spans,
                      span, scale);
   if (parts > 1 || spans) {
-    const int rows = parts > 1 ? a.Tk : a.S;
-    const int64_t blocks = (bks * rows * 2 * (D / 4) + 255) / 256;
+    const int rows = parts > 1 ? a.Tk : a.S, S = spans ? a.S : 0, wide = spans > 4 ? S : 0, per = 256 / (2 * D / 4);
+    const int64_t blocks = bks * wide + (bks * (rows - wide) + per - 1) / per;
     if (blocks >= (1ll << 31)) return 1;
     hipLaunchKernelGGL((window_sum_kernel<E, D>), dim3((unsigned)blocks), dim3(256), 0, st, (const float*)part, parts,
-                       spans, bks, rows, spans ? a.S : 0, a.Tk, (uint16_t*)dk, (uint16_t*)dv, scale);
+                       spans, bks, rows, S, wide, a.Tk, (uint16_t*)dk, (uint16_t*)dv, scale);
   }
   return (int)hipGetLastError();
 }

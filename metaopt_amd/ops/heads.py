@@ -311,13 +311,13 @@ def window_attention_ref(q, k, v, window=None, sinks=0, scale=None, start=None, 
     return o.reshape(B, H, Tq, D).permute(0, 2, 1, 3).reshape(B * Tq, H * D).to(q.dtype)
 
 
-def _span(window: int, sinks: int, heads: int, Tq: int) -> int:
+def _span(sinks: int, heads: int, Tq: int) -> int:
     """Queries of one item of the dK / dV kernel that adds up sinks' pairs out of the window
-    (csrc/lm_window.hip): 512 where these items fill the CUs (125M step: 91 us, with 128 117), else
-    about as many as an item within the window has (a window of 100, 14 key heads: 20 us, with 512
-    31); and so many that the 4 partial sums of the sinks' rows that each leaves are no more than
-    there are queries."""
-    near = 512 if heads * -(-Tq // 512) >= 512 else max(128, min(512, -(-window // 64) * 64))
+    (csrc/lm_window.hip): 512 where there are so many of these that they fill the CUs (125M step: 91
+    us, with 128 117), else 128, as the others wait for the last of them (8192 tokens, 4 key heads of
+    128: 189 us, with 512 225); and so many that the 4 partial sums of the sinks' rows that each
+    leaves are no more than there are queries."""
+    near = 512 if heads * -(-Tq // 512) >= 256 else 128
     return max(near, -(-4 * sinks // 64) * 64)
 
 
@@ -355,12 +355,12 @@ def _window_fwd(q, k, v, window, sinks, scale, start, start0, lengths, train):
     return o, rest, lse
 
 
-def _parts(blocks: int, steps: int, D: int) -> int:
+def _parts(blocks: int, steps: int) -> int:
     """Workgroups that share the queries of each of ``blocks`` key blocks in the dK / dV kernel,
-    where there are fewer blocks than the CUs take at once (two each for heads of 64, 8192 tokens of
-    4 key heads, window 1024: 123 + 9 us against 167; one for heads of 128), each with 8 of the
-    block's ``steps`` groups of 32 queries at least.  Their sums are added up by another launch."""
-    return max(1, min((512 if D == 64 else 256) // max(1, blocks), steps // 8))
+    where there are fewer blocks than two a CU (8192 tokens of 4 key heads, window 1024: heads of 64
+    123 + 9 us against 167, of 128 189 + 14 against 226), each with 8 of the block's ``steps``
+    groups of 32 queries at least.  Their sums are added up by another launch."""
+    return max(1, min(512 // max(1, blocks), steps // 8))
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -382,9 +382,9 @@ class _WindowAttention(torch.autograd.Function):
         if not o.numel() or not Tk:
             return (dq.zero_(), dk.zero_(), dv.zero_()) + (None,) * 6
         dsum = torch.empty_like(lse)
-        span = _span(window, sinks, B * KV, Tq)
+        span = _span(sinks, B * KV, Tq)
         spans = -(-Tq // span) if sinks and Tk > window else 0
-        parts = _parts(B * KV * -(-Tk // 128), H // KV * (min(Tq, window + 128) // 32), D)
+        parts = _parts(B * KV * -(-Tk // 128), H // KV * (min(Tq, window + 128) // 32))
         part = None
         if parts > 1 or spans:
             rows = parts * (Tk if parts > 1 else sinks) + 4 * spans * sinks
