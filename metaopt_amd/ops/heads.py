@@ -12,6 +12,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+from functools import reduce
+from operator import or_
 from typing import Optional
 
 import torch
@@ -35,6 +37,7 @@ _lib.register_signatures({
 })
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
+_Strides6, _Strides9 = c_int64 * 6, c_int64 * 9
 #: longest sequence and cache of :func:`window_attention`
 MAX_LENGTH = 1 << 29
 
@@ -58,8 +61,9 @@ def _p(t: Optional[torch.Tensor]):
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """``t`` with contiguous 16-byte aligned rows (a copy only where it has none)."""
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]) or \
-            t.stride(-2) >= 1 << 24:           # (a tile's 64 rows are reached by 32-bit offsets)
+    s = t.stride()
+    if s[-1] != 1 or t.data_ptr() % 16 or reduce(or_, s[:-1]) % 8 or \
+            s[-2] >= 1 << 24:                  # (a tile's 64 rows are reached by 32-bit offsets)
         return t.contiguous() if not t.is_contiguous() else t.clone()
     return t
 
@@ -69,10 +73,10 @@ def _needs_grad(*tensors) -> bool:
 
 
 def _same(t: torch.Tensor, names: str, *others) -> None:
-    device = t.device
+    index = t.get_device()                       # (-1: the CPU)
     for i, o in enumerate(others):
-        if o.device != device:
-            raise ValueError(f"{names.split()[i]} is on {o.device}, the input on {device}")
+        if o.get_device() != index:
+            raise ValueError(f"{names.split()[i]} is on {o.device}, the input on {t.device}")
 
 
 def _once(backward):
@@ -162,7 +166,7 @@ def _qk_fwd(qkv, wq, wk, cos, sin, T, H, KV, eps, il, k, v, start, cap):
     R, (P, D) = qkv.shape[0], wq.shape
     q = torch.empty(R // T, H, T, D, dtype=qkv.dtype, device=qkv.device)
     if R:
-        strides = (c_int64 * 6)(*k.stride()[:3], *v.stride()[:3])
+        strides = _Strides6(*k.stride()[:3], *v.stride()[:3])
         _call(qkv, "mopt_qk_norm_rope_fwd", _p(qkv), qkv.stride(0), _p(wq), _p(wk), _p(cos), _p(sin),
               _p(start), _p(q), _p(k), _p(v), strides, R, T, H, KV, R // P, D, cos.shape[0], cap, eps,
               int(il), _TYPES[qkv.dtype])
@@ -247,7 +251,8 @@ def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=
         raise ValueError(f"the caches are {tuple(kcache.shape)}: {n} sequences of heads of {D}")
     if kcache.dtype != qkv.dtype or vcache.dtype != qkv.dtype:
         raise ValueError("the caches must be of qkv's type")
-    if any(s == 0 and m > 1 for c in (kcache, vcache) for s, m in zip(c.stride(), c.shape)) or \
+    ks, vs = kcache.stride(), vcache.stride()
+    if (0 in ks + vs and any(s == 0 and m > 1 for s, m in zip(ks + vs, kcache.shape * 2))) or \
             (kcache.numel() and kcache.data_ptr() == vcache.data_ptr()):
         raise ValueError("the caches are written: no expanded tensors, and not one for both")
     _same(qkv, "kcache vcache start", kcache, vcache, start)
@@ -255,8 +260,8 @@ def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=
     if not _hip(qkv, "qk_norm_rope"):
         return _cached_ref(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps, il)
     _check_kernel("qk_norm_rope_cached", qkv, D)
-    for name, c in (("kcache", kcache), ("vcache", vcache)):
-        if c.stride(3) != 1 or c.data_ptr() % 16 or any(s % 8 for s in c.stride()[:3]):
+    for name, c, s in (("kcache", kcache, ks), ("vcache", vcache, vs)):
+        if s[3] != 1 or c.data_ptr() % 16 or (s[0] | s[1] | s[2]) % 8:
             raise ValueError(f"{name} needs contiguous rows at multiples of 16 bytes: it is written "
                              "in place")
     if cap == 0:
@@ -322,7 +327,7 @@ def _span(sinks: int, heads: int, Tq: int) -> int:
 
 
 def _geometry(q, k, v):
-    return (c_int64 * 9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    return _Strides9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
 
 
 def _splits(heads: int, tokens: int) -> int:
