@@ -288,9 +288,9 @@ __device__ __forceinline__ void hide(f32x16& x, float with, int i, int k0, int l
 
 // Forward: one pass over the keys with a running reference and sum.  Heads of 64 (4 sequences of 12
 // heads, 4096 tokens, window 512: 51 us, 475 TFLOP/s) are bound by the vector work on the scores, on a
-// SIMD about 670 clocks a group of 32 x 32 pairs beside 256 of products; heads of 128 (8192 tokens of
-// 16 / 4 heads, window 1024: 101 us, 640 TFLOP/s) by LDS: 16 KB of fragments a group and wave, and a
-// third wave a SIMD (tiles of 32 keys) changes nothing.
+// SIMD about 670 clocks a group of 32 x 32 pairs, and 256 of products that hardly overlap with it: 940.
+// Heads of 128 (8192 tokens of 16 / 4 heads, window 1024: 101 us, 640 TFLOP/s) by both: 660 + 512
+// clocks of 1320, with 2 waves a SIMD or 3 (tiles of 32 keys).
 template <class E, int D>
 __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a, uint16_t* o, uint16_t* rest,
                                                                        float* lse) {
@@ -404,7 +404,8 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
 // (`rest`, written by the forward): with o alone its error adds to that of the rounded dS, and where
 // few keys are seen it is the larger one (a window of 4: 1.8 times the error of a once rounded dq
 // instead of 1.5).  125M step (64 x 12 heads, 512 tokens, window 128): 84 us, of which reading and
-// writing 350 MB is 65; heads of 128, 8192 tokens, window 1024: 137 us (705 TFLOP/s), LDS-bound as above.
+// writing 350 MB is 65; heads of 128, 8192 tokens, window 1024: 137 us (705 TFLOP/s),
+// products and vector work as above.
 template <class E, int D>
 __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, const uint16_t* o,
                                                                      const uint16_t* rest, const uint16_t* dout,
@@ -534,9 +535,9 @@ __device__ __forceinline__ u32x4 pieces(float v, int lane) {
 // What is not a key's whole sum is left in 32 bits: the near sums of all rows (parts > 1) or of rows
 // j < S, [part][b, hk][rows][2][D], and the far ones behind them, [span][wave][b, hk][S][2][D];
 // window_sum_kernel adds them.  125M step (64 x 12 heads, 512 tokens, window 128, 4 sinks): 94 us, bound
-// by the vector work on the scores (exp2, dS, packing) between the products; heads of 128, 8192 tokens,
-// window 1024: 225 us (570 TFLOP/s), bound by LDS: 40 KB of fragments a group of 32 x 32 pairs and wave,
-// the same time with one and two waves a SIMD.  (Two waves for each key, 8 a workgroup, were slower
+// by the vector work on the scores (exp2, dS, packing) and the products, which hardly overlap; 8192
+// tokens of 16 / 4 heads, window 1024: heads of 64 108 us, of 128 189 us (six such sequences 880: 147
+// each, 880 TFLOP/s).  (Two waves for each key, 8 a workgroup, were slower
 // everywhere: 125M step 272 us.)
 template <class E, int D>
 struct Dkv {
@@ -643,7 +644,8 @@ struct Dkv {
   __device__ __forceinline__ void step(int slot, int sub, bool all, int d0, uint32_t mine) {
     const uint32_t Qs = lds_at(lds.ring[slot][0]) + sub * 64 * D, Os = lds_at(lds.ring[slot][1]) + sub * 64 * D;
     // Both products start at what their rows' sums take off: a value of each row in three pieces, times
-    // ones.  (From LDS to the registers that need them the 2 x 16 values would be 8 reads of 1 KB.)
+    // ones.  (From LDS to the registers that need them the 2 x 16 values would be 8 reads of 1 KB: heads
+    // of 64, 8192 tokens of 4 key heads, window 1024: 123 us so, 110 this way.)
     const int own = 32 * sub + swap23(lane & 31);
     const u32x4 ones = {0x3F803F80, 0x3F803F80, 0x3F803F80, 0x3F803F80};
     f32x16 x = Bf16::mfma32(pieces(-lds.stat[slot][0][own] * rc, lane), ones, zero16());
