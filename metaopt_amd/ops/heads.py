@@ -416,7 +416,8 @@ def window_attention(q, k, v, window: Optional[int] = None, sinks: int = 0, scal
     before it.  Within a sequence all values must be finite: a score outside the mask counts as
     absent, but a value's infinity or NaN reaches the queries whose tiles it shares.
 
-    ``scale``: positive, default ``1 / sqrt(D)``.  Any strides (copied where rows are not contiguous
+    ``scale``: positive (within [1e-30, 1e30]), default ``1 / sqrt(D)``.  Scores and log-sums are kept
+    in 32 bits: beyond 2^16 in size their last bits are felt in the gradients.  Any strides (copied where rows are not contiguous
     at multiples of 16 bytes).  Differentiable in q, k and v, with sums in a fixed order."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError("q is [B, H, Tq, D], k and v are [B, KV, Tk, D]")
@@ -433,8 +434,8 @@ def window_attention(q, k, v, window: Optional[int] = None, sinks: int = 0, scal
     if sinks < 0:
         raise ValueError(f"sinks {sinks} must not be negative")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f"scale {scale} must be positive")
+    if not 1e-30 <= scale <= 1e30:               # (its reciprocal is taken in 32 bits, too)
+        raise ValueError(f"scale {scale} must be positive, within [1e-30, 1e30]")
     if max(Tq, Tk) > MAX_LENGTH:
         raise ValueError(f"sequences and caches hold at most {MAX_LENGTH} tokens")
     _same(q, "k v", k, v)

@@ -240,7 +240,7 @@ def test_qk_norm_rope_cached_refuses(bad, match):
     (dict(q=torch.zeros(1, 3, 4, 8)), "multiple"), (dict(q=torch.zeros(2, 2, 4, 8)), "fit"),
     (dict(q=torch.zeros(2, 4, 8)), "B, H"), (dict(q=torch.zeros(1, 2, 4, 8).half()), "one type"),
     (dict(window=0), "window"), (dict(sinks=-1), "sinks"), (dict(scale=0.0), "positive"),
-    (dict(scale=float("inf")), "positive"), (dict(start=torch.zeros(1)), "int32"),
+    (dict(scale=float("inf")), "positive"), (dict(scale=1e-38), "positive"), (dict(start=torch.zeros(1)), "int32"),
     (dict(start=1 << 40), "position"), (dict(lengths=torch.zeros(2, dtype=torch.int32)), "int32"),
     (dict(lengths=torch.zeros(1, dtype=torch.int64)), "int32")])
 def test_window_attention_refuses(bad, match):

@@ -177,6 +177,9 @@ def _attention_oracle(q, k, v, do, window, sinks, start, lengths, scale=None):
     res = [(rows(o), rows(o_tol) + torch.finfo(q.dtype).tiny * u)]
     if do is None:
         return res
+    # the backward adds a score's products onto minus its row's log-sum (in base 2, at most the largest
+    # score's and the logarithm of the keys): a rounding of that size for each 16 of D, and two more
+    es = es + (D / 16 + 2) * F32 * (1.4427 * ((s * see).abs().amax() + math.log(Tk)) + 1)
     dod = torch.where(real, do.detach().double().view(B, Tq, H, D).transpose(1, 2).reshape(B, KV, G, Tq, D), zero)
     dv = (p.transpose(-1, -2) @ dod).sum(2)
     dv_tol = u * dv.abs() + (u + es) * (p.transpose(-1, -2) @ dod.abs()).sum(2)
@@ -310,6 +313,9 @@ def test_window_attention_large_scores_and_equal_scores():
     _check(q * 8, k * 8, v, do, 90, 4)
     _check(torch.zeros_like(q), k, v, do, 90, 4)
     _check(-k[:, :, :].clone() * 20, k * 20, v, do, 50, 0)
+    for scale in (1e-6, 1e-20, 4.0):
+        _check(*_attention_case(1, 2, 1, 300, 300, 64, FP), 90, 4, scale=scale)
+        _check(*_attention_case(1, 2, 1, 300, 300, 128, BF), 90, 4, scale=scale)
 
 
 def test_window_attention_is_deterministic_and_replays_in_a_graph():
