@@ -416,9 +416,10 @@ def window_attention(q, k, v, window: Optional[int] = None, sinks: int = 0, scal
     before it.  Within a sequence all values must be finite: a score outside the mask counts as
     absent, but a value's infinity or NaN reaches the queries whose tiles it shares.
 
-    ``scale``: positive (within [1e-30, 1e30]), default ``1 / sqrt(D)``.  Scores and log-sums are kept
-    in 32 bits: beyond 2^16 in size their last bits are felt in the gradients.  Any strides (copied where rows are not contiguous
-    at multiples of 16 bytes).  Differentiable in q, k and v, with sums in a fixed order."""
+    ``scale``: positive (within [1e-30, 1e30]), default ``1 / sqrt(D)``.  Scores and log-sums are
+    kept in 32 bits: beyond 2^16 in size their last bits are felt in the gradients.  Any strides
+    (copied where rows are not contiguous at multiples of 16 bytes).  Differentiable in q, k and v,
+    with sums in a fixed order."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError("q is [B, H, Tq, D], k and v are [B, KV, Tk, D]")
     B, H, Tq, D = q.shape
