@@ -179,13 +179,11 @@ def _prepare_window(c, g):
 
 def _prepare_distill(c, g):
     R, V, K = c["trials"] * c["rows"], c["vocab"], c["top"]
-    logits = _randn(g, R, V, scale=2.0)
+    logits = _randn(g, R, V, dtype=DTYPES[c["dtype"]], scale=2.0)
     index = torch.randint(0, V, (R, K), generator=g, device="cuda")
     top = _randn(g, R, K, scale=2.0, mean=6.0).sort(1, descending=True).values
-    # the student half agrees with its teacher (where a row has an index twice the larger value
-    # stays: one that does not go by the order of the writes)
-    logits.scatter_reduce_(1, index, 0.5 * top + _randn(g, R, K), "amax")
-    logits = logits.to(DTYPES[c["dtype"]])
+    # the student half agrees with its teacher
+    logits.scatter_(1, index, (0.5 * top + _randn(g, R, K)).to(logits.dtype))
     labels = index[:, 0].clone()
     if c["missing"]:
         cut = torch.rand(R, generator=g, device="cuda")
