@@ -238,7 +238,8 @@ int mopt_qk_norm_rope_fwd(const void* x, int64_t x_ld, const void* wq, const voi
                           const void* cosT, const void* sinT, const void* start, void* q, void* k,
                           void* v, const int64_t* kv_strides, int rows, int T, int H, int KV, int rpt,
                           int D, int reach, int cap, float eps, int il, int dtype, void* stream) {
-  if (rows <= 0 || T <= 0 || H <= 0 || KV <= 0 || rpt <= 0 || (D != 64 && D != 128) || cap <= 0) return 1;
+  if (rows <= 0 || T <= 0 || H <= 0 || KV <= 0 || rpt <= 0 || (D != 64 && D != 128)) return 1;
+  if (cap <= 0 || reach <= 0) return 1;      // (row 0 of the tables is read for a token without a position)
   if (!start && (cap < T || reach < T)) return 1;
   if (((int64_t)rows * (H + 2 * KV) * D) / 2048 >= (1ll << 31) - 1) return 1;
   const QkArgs a{(const uint16_t*)x, x_ld, (const uint16_t*)wq, (const uint16_t*)wk,

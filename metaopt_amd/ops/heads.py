@@ -264,7 +264,7 @@ def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=
         if s[3] != 1 or c.data_ptr() % 16 or (s[0] | s[1] | s[2]) % 8:
             raise ValueError(f"{name} needs contiguous rows at multiples of 16 bytes: it is written "
                              "in place")
-    if cap == 0:
+    if cap == 0 or not len(cos):
         return torch.zeros(n, H, T, D, dtype=qkv.dtype, device=qkv.device)
     return _qk_fwd(_rows16(qkv), _dense16(wq), _dense16(wk), cos, sin, T, H, KV, float(eps), il,
                    kcache, vcache, start, cap)
@@ -273,6 +273,8 @@ def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=
 @torch.no_grad()
 def _cached_ref(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps, il):
     n, KV, cap = kcache.shape[:3]
+    if cap == 0 or not len(cos):                 # no token has a place
+        return qkv.new_zeros(n, H, T, wq.shape[1])
     at = start.long()[:, None] + torch.arange(T, device=qkv.device)
     ok = (at >= 0) & (at < min(cap, cos.shape[0]))
     rows = torch.where(ok, at, torch.zeros_like(at)).reshape(-1)     # the tables' rows, one a token

@@ -1,11 +1,12 @@
 """ops.heads and ops.distill on the CPU: the references against loops over their definitions, their
 gradients against differences, and what the entry points refuse."""
+import ctypes
 import math
 
 import pytest
 import torch
 
-from metaopt_amd.ops import distill, heads, lm
+from metaopt_amd.ops import _lib, distill, heads, lm
 
 
 def _rand(*shape, dtype=torch.float64):
@@ -266,3 +267,32 @@ def test_distill_loss_refuses(bad, match):
              rows_per_trial=2)
     with pytest.raises(ValueError, match=match):
         distill.distill_loss(**dict(d, **bad))
+
+
+def test_cached_heads_with_tables_of_no_position():
+    """No position is inside tables that hold none: nothing is written, every query is 0."""
+    kc, vc = torch.full((2, 2, 4, 8), 9.0), torch.full((2, 2, 4, 8), 9.0)
+    cos, sin = heads.rope_tables(0, 8)
+    q = heads.qk_norm_rope_cached(torch.ones(4, 48), torch.ones(1, 8), torch.ones(1, 8), cos, sin, 2, 2, kc, vc,
+                                  torch.zeros(2, dtype=torch.int32))
+    assert tuple(q.shape) == (2, 2, 2, 8) and not q.any()
+    assert (kc == 9).all() and (vc == 9).all()
+
+
+def test_cached_heads_do_not_launch_with_tables_of_no_position(monkeypatch):
+    """The kernel reads row 0 of the tables for a token that has no position."""
+    monkeypatch.setattr(heads, "_hip", lambda t, op="": True)
+    monkeypatch.setattr(heads, "_call", lambda *args: pytest.fail("launched"))
+    rows, w = torch.ones(4, 384, dtype=torch.bfloat16), torch.ones(1, 64, dtype=torch.bfloat16)
+    caches = [torch.full((2, 2, 4, 64), 9.0, dtype=torch.bfloat16) for _ in "kv"]
+    cos, sin = heads.rope_tables(0, 64)
+    q = heads.qk_norm_rope_cached(rows, w, w, cos, sin, 2, 2, *caches, torch.zeros(2, dtype=torch.int32))
+    assert tuple(q.shape) == (2, 2, 2, 64) and not q.any() and all((c == 9).all() for c in caches)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses of nothing: only where nothing can be launched")
+def test_the_kernel_s_entry_refuses_tables_of_no_position():
+    one = ctypes.c_int32(0)
+    args = [None, 384, None, None, None, None, ctypes.addressof(one), None, None, None, heads._Strides6(), 4, 2, 2, 2,
+            4, 64, 0, 4, 1e-5, 0, 0, None]
+    assert _lib.get_lib().mopt_qk_norm_rope_fwd(*args) == 1      # (1: refused on the host, in front of the launch)

@@ -381,3 +381,14 @@ def test_offsets_past_32_bits():
     assert torch.equal(v[:, :, Tk - 1], kc[2][:, :, 0])
     assert torch.equal(k[:, :, Tk - 1], kc[1][:, :, 0])          # (the angle of every row is 0)
     assert not v[:, :, :Tk - 1].any()
+
+
+def test_cached_heads_with_tables_of_no_position():
+    """Every token is outside tables that hold no position: zeros, and the caches stay."""
+    rows, w = _rand(4, 6 * 64, dtype=BF), torch.ones(1, 64, device=DEV, dtype=BF)
+    caches = [_rand(2, 2, 4, 64, dtype=BF) for _ in "kv"]
+    before = [c.clone() for c in caches]
+    start = torch.zeros(2, dtype=torch.int32, device=DEV)
+    q = heads.qk_norm_rope_cached(rows, w, w, *heads.rope_tables(0, 64, device=DEV), 2, 2, *caches, start)
+    assert tuple(q.shape) == (2, 2, 2, 64) and not q.any()
+    assert all(torch.equal(a, b) for a, b in zip(caches, before))
