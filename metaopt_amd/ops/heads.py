@@ -283,7 +283,7 @@ def _cached_ref(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps, il):
     b, t = ok.nonzero(as_tuple=True)
     kcache[b, :, at[b, t]] = k[b, :, t]
     vcache[b, :, at[b, t]] = v[b, :, t]
-    return q * ok[:, None, :, None]
+    return torch.where(ok[:, None, :, None], q, torch.zeros_like(q))
 
 
 # ============================================================================ window attention

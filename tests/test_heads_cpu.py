@@ -296,3 +296,12 @@ def test_the_kernel_s_entry_refuses_tables_of_no_position():
     args = [None, 384, None, None, None, None, ctypes.addressof(one), None, None, None, heads._Strides6(), 4, 2, 2, 2,
             4, 64, 0, 4, 1e-5, 0, 0, None]
     assert _lib.get_lib().mopt_qk_norm_rope_fwd(*args) == 1      # (1: refused on the host, in front of the launch)
+
+
+def test_cached_heads_of_tokens_without_a_position_are_zero_whatever_the_row_holds():
+    rows = torch.full((2, 48), float("nan"))
+    cos, sin = heads.rope_tables(4, 8)
+    kc, vc = torch.zeros(2, 2, 4, 8), torch.zeros(2, 2, 4, 8)
+    q = heads.qk_norm_rope_cached(rows, torch.ones(1, 8), torch.ones(1, 8), cos, sin, 1, 2, kc, vc,
+                                  torch.tensor([4, -1], dtype=torch.int32))
+    assert (q == 0).all() and not kc.any() and not vc.any()
