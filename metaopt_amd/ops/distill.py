@@ -9,7 +9,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .heads import _call, _once, _p, _same
+from .heads import _call, _no_tangents, _once, _p, _same
 from .lm import _hip, _ScaledGrad
 
 c_void_p, c_int, c_float, c_int64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
@@ -157,6 +157,7 @@ def distill_loss(logits, labels, top_values, top_index, rows_per_trial, temperat
         if t.dtype not in _TYPES:
             raise ValueError(f"distill_loss on a GPU takes bfloat16, float16 or float32 {name}, not "
                              f"{t.dtype}")
+    _no_tangents("distill_loss", logits, top_values, *(t for t in (tau, alpha) if torch.is_tensor(t)))
     if R == 0:
         return logits.new_zeros(P, dtype=torch.float32) + 0.0 * logits.sum()
     need = torch.is_grad_enabled() and logits.requires_grad

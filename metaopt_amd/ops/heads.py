@@ -17,6 +17,7 @@ from operator import or_
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .lm import _hip
@@ -70,6 +71,16 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 
 def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+def _no_tangents(what: str, *tensors) -> None:
+    """The kernels carry no forward-mode derivatives.  (A dual tensor need not require a gradient:
+    its tangent would be lost without a word.)"""
+    if getattr(forward_ad, "_current_level", 0) < 0:       # out of dual_level(): the cheap way out
+        return
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} on a GPU has no forward-mode derivatives")
 
 
 def _same(t: torch.Tensor, names: str, *others) -> None:
@@ -231,6 +242,7 @@ def qk_norm_rope(qkv, wq, wk, cos, sin, T, H, kv_heads=None, eps=1e-5, il=False)
     if not _hip(qkv, "qk_norm_rope"):
         return qk_norm_rope_ref(qkv, wq, wk, cos, sin, T, H, KV, eps, il)
     _check_kernel("qk_norm_rope", qkv, D)
+    _no_tangents("qk_norm_rope", qkv, wq, wk, cos, sin)
     args = _rows16(qkv), _dense16(wq), _dense16(wk), cos, sin, T, H, KV, float(eps), bool(il)
     return _QKNormRope.apply(*args) if _needs_grad(qkv, wq, wk) else _qk_heads(*args)
 
@@ -260,6 +272,7 @@ def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=
     if not _hip(qkv, "qk_norm_rope"):
         return _cached_ref(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps, il)
     _check_kernel("qk_norm_rope_cached", qkv, D)
+    _no_tangents("qk_norm_rope_cached", qkv, wq, wk, cos, sin, kcache, vcache)
     for name, c, s in (("kcache", kcache, ks), ("vcache", vcache, vs)):
         if s[3] != 1 or c.data_ptr() % 16 or (s[0] | s[1] | s[2]) % 8:
             raise ValueError(f"{name} needs contiguous rows at multiples of 16 bytes: it is written "
@@ -457,6 +470,7 @@ def window_attention(q, k, v, window: Optional[int] = None, sinks: int = 0, scal
         return window_attention_ref(q, k, v, window, sinks, scale, start0 if start is None else start,
                                     lengths)
     _check_kernel("window_attention", q, D)
+    _no_tangents("window_attention", q, k, v)
     # a window over all positions is no window; sinks within every window are none
     reach = 1 << 30 if window is None else min(int(window), 1 << 30)
     sinks = min(int(sinks), Tk) if reach < Tk else 0

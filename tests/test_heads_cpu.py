@@ -305,3 +305,63 @@ def test_cached_heads_of_tokens_without_a_position_are_zero_whatever_the_row_hol
     q = heads.qk_norm_rope_cached(rows, torch.ones(1, 8), torch.ones(1, 8), cos, sin, 1, 2, kc, vc,
                                   torch.tensor([4, -1], dtype=torch.int32))
     assert (q == 0).all() and not kc.any() and not vc.any()
+
+
+# ------------------------------------------------------------------------------- forward mode
+def _forward_mode_calls():
+    """(name, call of one tensor, the tensor): each differentiable argument of the operators."""
+    torch.manual_seed(12)
+    bf = torch.bfloat16
+    cos, sin = heads.rope_tables(2, 64)
+    qkv, w = _rand(4, 384, dtype=bf), _rand(1, 64, dtype=bf)
+    start = torch.zeros(2, dtype=torch.int32)
+    caches = [_rand(2, 2, 4, 64, dtype=bf) for _ in "kv"]
+    q, k = _rand(1, 2, 4, 64, dtype=bf), _rand(1, 1, 4, 64, dtype=bf)
+    x, top = _rand(4, 9, dtype=torch.float32), _rand(4, 3, dtype=torch.float32)
+    y, index = torch.zeros(4, dtype=torch.int32), torch.arange(12, dtype=torch.int32).view(4, 3) % 9
+    tau, alpha = torch.ones(2), torch.full((2,), 0.5)
+
+    def rope(qkv=qkv, wq=w, wk=w, cos=cos, sin=sin):
+        return heads.qk_norm_rope(qkv, wq, wk, cos, sin, 2, 2)
+
+    def cached(qkv=qkv, wq=w, wk=w, cos=cos, sin=sin, kc=caches[0], vc=caches[1]):
+        return heads.qk_norm_rope_cached(qkv, wq, wk, cos, sin, 2, 2, kc, vc, start)
+
+    def attention(q=q, k=k, v=k):
+        return heads.window_attention(q, k, v, 2, 1)
+
+    def loss(x=x, top=top, tau=tau, alpha=alpha):
+        return distill.distill_loss(x, y, top, index, 2, tau, alpha)
+    for f, args in ((rope, dict(qkv=qkv, wq=w, wk=w, cos=cos, sin=sin)),
+                    (cached, dict(qkv=qkv, wq=w, wk=w, cos=cos, sin=sin, kc=caches[0], vc=caches[1])),
+                    (attention, dict(q=q, k=k, v=k)), (loss, dict(x=x, top=top, tau=tau, alpha=alpha))):
+        for name, t in args.items():
+            yield f"{f.__name__}-{name}", (lambda t, f=f, name=name: f(**{name: t})), t
+
+
+CALLS = {name: (call, t) for name, call, t in _forward_mode_calls()}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_kernels_refuse_forward_mode_derivatives(name, monkeypatch):
+    """A dual tensor does not require a gradient: a call that looks at that alone would drop its
+    tangent, which counts as a derivative of 0."""
+    call, t = CALLS[name]
+    for module in (heads, distill):
+        monkeypatch.setattr(module, "_hip", lambda t, op="": True)
+        monkeypatch.setattr(module, "_call", lambda *args: pytest.fail("launched"))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(dual)
+
+
+def test_references_have_forward_mode_derivatives():
+    torch.manual_seed(13)
+    q, d = _rand(1, 2, 4, 8), _rand(1, 2, 4, 8)
+    with torch.autograd.forward_ad.dual_level():
+        o = heads.window_attention(torch.autograd.forward_ad.make_dual(q, d), q, q, 2, 1)
+        got = torch.autograd.forward_ad.unpack_dual(o).tangent
+    h = 1e-6
+    ends = [heads.window_attention(q + s * d, q, q, 2, 1) for s in (h, -h)]
+    torch.testing.assert_close(got, (ends[0] - ends[1]) / (2 * h), rtol=1e-6, atol=1e-8)

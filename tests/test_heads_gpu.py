@@ -392,3 +392,13 @@ def test_cached_heads_with_tables_of_no_position():
     q = heads.qk_norm_rope_cached(rows, w, w, *heads.rope_tables(0, 64, device=DEV), 2, 2, *caches, start)
     assert tuple(q.shape) == (2, 2, 2, 64) and not q.any()
     assert all(torch.equal(a, b) for a, b in zip(caches, before))
+
+
+def test_forward_mode_is_refused():
+    """(a dual tensor does not require a gradient, and its tangent must not get lost)"""
+    q = _rand(1, 2, 4, 64, dtype=BF)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            heads.window_attention(dual, q, q)
+        heads.window_attention(q, q, q)
