@@ -26,7 +26,8 @@ struct Bf16 {
 
 struct Fp16 {
   // Probabilities of a long context lie among the subnormal fp16 values (below 2^-14, where a
-  // rounding is no longer relative): the backward products take them 2^12 times as large.
+  // rounding is no longer relative): the backward products take them 2^12 times as large.  (Score
+  // gradients go with the incoming gradient's size: lm_window.hip scales them as they come.)
   static constexpr int kShift = 12;
   static __device__ __forceinline__ float up(uint32_t h) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)h);

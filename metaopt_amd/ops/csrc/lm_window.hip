@@ -286,6 +286,28 @@ __device__ __forceinline__ void hide(f32x16& x, float with, int i, int k0, int l
   }
 }
 
+// Score gradients dS on their way into fp16.  Those of a mean loss over many tokens are far below 2^-14,
+// where fp16 has multiples of 2^-24 only, and a fixed factor that lifts these lets others overflow.  So
+// each row of a product (dQ: a query, dK: a key) carries a power of two of its own: dS comes multiplied by
+// it, and where a row's largest passes 2^15 the factor, this group and the sums so far are brought down to
+// put it at 2^7 ... 2^8.  A pair is then off by 2^-11 of itself or 2^-32 of its row's largest.  It starts at
+// 2^60: products of fp16 rows (below 2^39) stay inside 32 bits with it.
+constexpr float kFirstLift = (float)(1ull << 60);
+
+// the factor that `x`, its row's sums and its lift take now (1, mostly)
+template <class E>
+__device__ __forceinline__ float settle(f32x16& x) {
+  float mx = fabsf(x[0]);
+#pragma unroll
+  for (int r = 1; r < 16; ++r) mx = fmaxf(mx, fabsf(x[r]));
+  mx = other_half(mx, true);
+  if (!__any(mx > 32768.f)) return 1.f;
+  const float f = mx > 32768.f ? __uint_as_float((261u - (__float_as_uint(mx) >> 23)) << 23) : 1.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] *= f;
+  return f;
+}
+
 // Forward: one pass over the keys with a running reference and sum.  Heads of 64 (4 sequences of 12
 // heads, 4096 tokens, window 512: 51 us, 475 TFLOP/s) are bound by the vector work on the scores, on a
 // SIMD about 670 clocks a group of 32 x 32 pairs, and 256 of products that hardly overlap with it: 940.
@@ -430,7 +452,7 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
   f32x16 acc[DN];
 #pragma unroll
   for (int dn = 0; dn < DN; ++dn) acc[dn] = zero16();
-  float ds = 0.f;
+  float ds = 0.f, lift = E::kShift ? kFirstLift : 1.f;
   uint16_t* img = ring[0][0] + wave * Rows<D>::SIZE;
   if (bt0 <= bt1) {
     const uint16_t* kg = a.k + b * a.k_sb + hk * a.k_sh;
@@ -488,7 +510,8 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
       };
       auto slope = [&](f32x16& x, const f32x16& y) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.c, -ls)) * (y[r] - ds);
+        for (int r = 0; r < 16; ++r)
+          x[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.c, -ls)) * (E::kShift ? fmaf(y[r], lift, -ds * lift) : y[r] - ds);
       };
       auto add = [&](const f32x16& x, int sub) {
 #pragma unroll
@@ -507,12 +530,20 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
         scores(sub, x, y);
         slope(x, y);
         if (see == 1) hide<E>(x, 0.f, i, k0, lane, a.W, a.S);
+        if constexpr (E::kShift) {
+          const float f = settle<E>(x);
+          if (__any(f != 1.f)) {
+            lift *= f;
+#pragma unroll
+            for (int dn = 0; dn < DN; ++dn) acc[dn] *= f;
+          }
+        }
         add(x, sub);
       }
     }
   }
   __syncthreads();
-  Rows<D>::template put<E, false>(acc, valid ? scale : 0.f, dq + (int64_t)bh * a.Tq * D, D, tw, 0, a.Tq, img, lane);
+  Rows<D>::template put<E, false>(acc, valid ? scale / lift : 0.f, dq + (int64_t)bh * a.Tq * D, D, tw, 0, a.Tq, img, lane);
   if (lane < 32) dsum[(int64_t)bh * nqb * BM + t] = valid ? ds : 0.f;
 }
 
@@ -562,8 +593,10 @@ struct Dkv {
   Fill<D, QN> qfill, ofill;
   u32x4 kf[DK], vf[kValuesInLds ? 1 : DK];
   f32x16 ak[DN], av[DN];
+  float lift;                                          // of this lane's key, over 2^kShift; fp16
 
   __device__ __forceinline__ void clear() {
+    lift = kFirstLift * kUnshift;
 #pragma unroll
     for (int dn = 0; dn < DN; ++dn) ak[dn] = av[dn] = zero16();
   }
@@ -589,6 +622,9 @@ struct Dkv {
       sn += tq_pad;
     }
   }
+
+  // what takes the lift off ak
+  __device__ __forceinline__ float plain() const { return E::kShift ? kUnshift / lift : 1.f; }
 
   // Tiles [it0, it1) of those of rows [tb, te) of each query head, for the pairs with
   // lo <= i - j < lo + n: the window's (0, W), or far ones (W, as many as there may be; j < S)
@@ -677,7 +713,15 @@ struct Dkv {
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) y[r] *= E::kShift ? x[r] * kUnshift : x[r];
+    for (int r = 0; r < 16; ++r) y[r] *= E::kShift ? x[r] * lift : x[r];
+    if constexpr (E::kShift) {
+      const float f = settle<E>(y);
+      if (__any(f != 1.f)) {
+        lift *= f;
+#pragma unroll
+        for (int dn = 0; dn < DN; ++dn) ak[dn] *= f;
+      }
+    }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const u32x4 p = pack<E>(x, st);
@@ -693,12 +737,14 @@ struct Dkv {
   }
 
   __device__ __forceinline__ void put_part(float* dst) const {
+    const float f = plain();
 #pragma unroll
     for (int dn = 0; dn < DN; ++dn)
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         const int col = 32 * dn + 8 * r4 + 4 * (lane >> 5);
-        *(f32x4*)(dst + col) = f32x4{ak[dn][4 * r4], ak[dn][4 * r4 + 1], ak[dn][4 * r4 + 2], ak[dn][4 * r4 + 3]};
+        const f32x4 k4 = {ak[dn][4 * r4], ak[dn][4 * r4 + 1], ak[dn][4 * r4 + 2], ak[dn][4 * r4 + 3]};
+        *(f32x4*)(dst + col) = E::kShift ? k4 * f : k4;
         *(f32x4*)(dst + D + col) = f32x4{av[dn][4 * r4], av[dn][4 * r4 + 1], av[dn][4 * r4 + 2], av[dn][4 * r4 + 3]};
       }
   }
@@ -750,7 +796,7 @@ __global__ __launch_bounds__(256, kDkvWaves<D>) void window_dkv_kernel(
   if (parts == 1) {
     const int64_t base = (int64_t)bk * a.Tk * D;
     const int lo = spans ? a.S : 0;
-    Rows<D>::template put<E, false>(k.ak, scale, dk + base, D, kw, lo, a.Tk, img, lane);
+    Rows<D>::template put<E, false>(k.ak, scale * k.plain(), dk + base, D, kw, lo, a.Tk, img, lane);
     Rows<D>::template put<E, false>(k.av, K::kUnshift, dv + base, D, kw, lo, a.Tk, img, lane);
   }
   if (some && j < a.Tk) k.put_part(part + ((c * bks + bk) * rows + j) * 2 * D);

@@ -402,3 +402,57 @@ def test_forward_mode_is_refused():
         with pytest.raises(NotImplementedError, match="forward-mode"):
             heads.window_attention(dual, q, q)
         heads.window_attention(q, q, q)
+
+
+def _eighths(*shape, most):
+    """fp16 values that are multiples of 1/8 of at most ``most``: exact at any power of two in range."""
+    return (torch.randn(*shape, device=DEV) * 8).round().clamp(-8 * most, 8 * most).div(8).half()
+
+
+@pytest.mark.parametrize("B,H,KV,T,D,window,sinks", [
+    (2, 3, 3, 300, 64, 100, 4), (1, 4, 1, 300, 128, None, 0), (1, 4, 2, 1100, 64, 100, 4), (1, 4, 1, 1300, 128, 1000, 2),
+    (1, 2, 2, 40, 64, None, 0)])
+@pytest.mark.parametrize("power", [-13, -10, 8])
+def test_window_attention_fp16_gradients_follow_the_incoming_size(power, B, H, KV, T, D, window, sinks):
+    """Gradients are linear in the output's: do 2^power gives 2^power of what do gives, exactly before the
+    last rounding, if score gradients lose nothing on the way whatever their size.  That rounding is off by
+    u of the value or, in the subnormal range, by 2^-25, once on either side.
+
+    (Scores 8 q k / 64 of size 1; queries, keys and 8 / 64 leave gradients of a size of about 1 for do of
+    size 1, so at 2^-13 a score gradient is about 2^-20, the gradients about 2^-13.)"""
+    torch.manual_seed(T + D)
+    q, k, v = (_rand(B, h, T, D, dtype=FP, scale=s) for h, s in ((H, 0.125), (KV, 0.125), (KV, 1.0)))
+    do = _eighths(B * T, H * D, most=4)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = heads.window_attention(*leaves, window, sinks, scale=8.0)
+    want, got = (torch.autograd.grad(o, leaves, d, retain_graph=True) for d in (do, do * 2.0 ** power))
+    assert torch.equal(do * 2.0 ** power * 2.0 ** -power, do)
+    for g, w, name in zip(got, want, ("dq", "dk", "dv")):
+        w, back = w.double(), g.double() * 2.0 ** -power
+        tol = 2 * _u(FP) * w.abs() * (1 + _u(FP)) + 2.0 ** -25 * (1 + 2.0 ** -power)
+        _within(back, w, tol, name)
+
+
+@pytest.mark.parametrize("D,T,window", [(64, 700, 90), (128, 900, 200)])
+def test_window_attention_fp16_gradients_of_rows_of_unlike_sizes(D, T, window):
+    """Rows of do of 1 and of 2^-13 in one sequence: dq of the small ones, and dk of keys that only these
+    see, are what they are where all rows are small."""
+    torch.manual_seed(T)
+    q, k, v = (_rand(1, 2, T, D, dtype=FP, scale=s) for s in (0.125, 0.125, 1.0))
+    do = _eighths(T, 2 * D, most=4)
+    small, mixed = do * 2.0 ** -13, do.clone()
+    mixed[:T // 2] *= 2.0 ** -13
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = heads.window_attention(*leaves, window, scale=8.0)
+    a, b = (torch.autograd.grad(o, leaves, d, retain_graph=True) for d in (mixed, small))
+    cut = T // 2 - window                           # keys seen by queries in front of T / 2 only
+    assert torch.equal(a[0][:, :, :T // 2], b[0][:, :, :T // 2])
+    assert torch.equal(a[1][:, :, :cut], b[1][:, :, :cut]) and a[1][:, :, :cut].any()
+    assert torch.equal(a[2][:, :, :cut], b[2][:, :, :cut])
+
+
+@pytest.mark.parametrize("T", [60, 500])
+def test_window_attention_fp16_large_score_gradients(T):
+    """Score gradients past fp16's largest value (65504), whose sums of products over 16 are not."""
+    q, k, v, do = _attention_case(1, 2, 2, T, T, 64, FP)
+    _check(q, k, (v * 32).half(), (do * 256).half(), 50, 2, scale=0.0625)
