@@ -22,7 +22,7 @@ using namespace mopt;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct F32 {};
 
@@ -185,8 +185,10 @@ __global__ __launch_bounds__(NT, WAVES) void distill_row_kernel(DistillArgs a) {
   });
   block_all<NT, 2, true>(mx, red);
   const float m = mx[0], tm = mx[1];
-  // (the reference is in the exponent's fma: what its rounding changes is a factor of all terms)
-  const float k1 = kLog2e, kt = kLog2e * rtau, b1 = -m * k1, bt = -m * kt;
+  // Exponents are formed from v - m itself, the reference that the loss is relative to: with -m k rounded
+  // once and added in an fma, all terms are off by one factor that the loss does not take off again (losses
+  // of rows with logits of 1000: 4e-5 off; past m / tau = 2^31 the factor is infinite).
+  const float kt = kLog2e * rtau;
   const bool hard = has_label && alpha != 1.f, soft = tm > -INFINITY && alpha != 0.f;
   char* const g = (char*)a.grad + row * (int64_t)V * R::SIZE;
   if (!hard && !soft) {                              // no loss and no gradient, whatever the logits are
@@ -199,8 +201,8 @@ __global__ __launch_bounds__(NT, WAVES) void distill_row_kernel(DistillArgs a) {
   }
   float sums[4] = {0.f, 0.f, 0.f, 0.f};            // z1, ztau, zq, sum e_k (log e_k - x_k / tau)
   auto add = [&](float v) {
-    sums[0] += __builtin_amdgcn_exp2f(fmaf(v, k1, b1));
-    sums[1] += __builtin_amdgcn_exp2f(fmaf(v, kt, bt));
+    sums[0] += __builtin_amdgcn_exp2f((v - m) * kLog2e);
+    sums[1] += __builtin_amdgcn_exp2f((v - m) * kt);
   };
   each([&](int, const float (&f)[N]) {
 #pragma unroll
@@ -228,7 +230,7 @@ __global__ __launch_bounds__(NT, WAVES) void distill_row_kernel(DistillArgs a) {
   const float h1 = hard ? scale * (1.f - alpha) : 0.f, ht = soft ? scale * alpha * tau : 0.f;
   const float c1 = hard ? h1 / sums[0] : 0.f, ct = soft ? ht / sums[1] : 0.f;
   auto dense = [&](float v) {
-    return fmaf(c1, __builtin_amdgcn_exp2f(fmaf(v, k1, b1)), ct * __builtin_amdgcn_exp2f(fmaf(v, kt, bt)));
+    return fmaf(c1, __builtin_amdgcn_exp2f((v - m) * kLog2e), ct * __builtin_amdgcn_exp2f((v - m) * kt));
   };
   // The corrected places, each computed by the entries that have it (the teacher's, then the
   // label).  Their logits are read before any gradient is written: it may take the logits' place.

@@ -184,3 +184,71 @@ def test_distill_empty_and_refusals():
     with pytest.raises(ValueError, match="float64"):
         distill.distill_loss(torch.zeros(2, 5, device=DEV).double(), torch.zeros(2, dtype=torch.int32, device=DEV),
                              torch.zeros(2, 2, device=DEV), torch.zeros(2, 2, dtype=torch.int32, device=DEV), 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("offset", [0.0, 24.0, -24.0, 1000.0, -1000.0, 30000.0, -30000.0])
+def test_distill_loss_of_shifted_logits(offset, dtype):
+    """Rows of which one logit stands out by 6 to 16, all shifted by ``offset``: the loss does not go with
+    it.  (fp16 logits at 1000 and 30000 are multiples of 1/2 and 16: what they are is what counts.)
+
+    z, the sum of exponentials relative to the largest logit m, is 1 and a rest: at most 17 values of a thread
+    and 10 more sums round to 2^-24 of about 1, an exponential e^d is off by (2 |d| + 4) 2^-24 of itself.
+    log z and x - m are rounded, and their difference."""
+    torch.manual_seed(5)
+    R, V, K, tau = 64, 1001, 6, 2.0
+    x = torch.randn(R, V, device=DEV)
+    y = torch.randint(0, V, (R,), device=DEV, dtype=torch.int32)
+    x[torch.arange(R, device=DEV), y.long()] = torch.linspace(9, 19, R, device=DEV)
+    x = (x + offset).to(dtype)
+    index = torch.randint(0, V, (R, K), device=DEV, dtype=torch.int32)
+    index[:, 0] = y
+    top = torch.randn(R, K, device=DEV)
+    top[:, 0] += 8
+    d = x.double() - x.double().amax(1, keepdim=True)
+    f, exp = 2.0 ** -24, lambda a: a.exp() * (2 * a.abs() + 4)  # noqa: E731
+
+    def log_sum(a):
+        z = a.exp().sum(1)
+        return z.log(), f * (27 * z + exp(a).sum(1) - 4 + 2 * z.log().abs()) / z
+    lz, tol = log_sum(d)
+    dy = d.gather(1, y.long()[:, None])[:, 0]
+    want, tol = lz - dy, tol + f * (2 * dy.abs() + 2 * (lz - dy).abs())
+    with torch.no_grad():
+        got = distill.distill_loss(x, y, top, index, 1, tau, 0.0).double()
+    assert (got >= 0).all()
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max().item()
+    # the teacher's: q_k = e^t_k / z_q, sum q_k (t_k - (x_k - m) / tau) - log z_q + log z_tau
+    lt, tol = log_sum(d / tau)
+    t = (top.double() - top.double().amax(1, keepdim=True)) / tau
+    lq, tol_q = log_sum(t)
+    part = t - d.gather(1, index.long()) / tau
+    q = t.softmax(1)
+    want = tau * tau * ((q * part).sum(1) - lq + lt)
+    tol = tol + tol_q + f * ((q * part.abs() * (2 * t.abs() + 4 + 16)).sum(1) + (q * (t.abs() + part.abs()) * 4).sum(1)
+                             + 2 * (lq.abs() + lt.abs() + (q * part).sum(1).abs()))
+    with torch.no_grad():
+        got = distill.distill_loss(x, y, top, index, 1, tau, 1.0).double()
+    assert ((got - want).abs() <= tau * tau * tol).all(), ((got - want).abs() / (tau * tau * tol)).max().item()
+
+
+def test_distill_loss_of_a_low_temperature_and_far_logits():
+    """m / tau past 2^31: sums, losses and gradients are those of the differences to the largest logit."""
+    x = 10000.0 + torch.randn(8, 500, device=DEV)
+    y = torch.zeros(8, device=DEV, dtype=torch.int32)
+    index = x.topk(3, 1).indices.int()
+    top = torch.zeros(8, 3, device=DEV)
+    leaf = x.requires_grad_(True)
+    loss = distill.distill_loss(leaf, y, top, index, 8, 1e-6, 0.5)
+    g, = torch.autograd.grad(loss.sum(), leaf)
+    with torch.no_grad():
+        alone = distill.distill_loss(leaf[:, :], y, top, index, 8, 1e-6, 0.0)
+    # the student at this temperature is its largest logit alone: a tau (1 - 1 / 3), and -a tau / 3 twice
+    assert torch.isfinite(loss).all() and torch.isfinite(g).all()
+    soft = 0.5 * 1e-6 * (2.0 / 3)
+    hard = 0.5 * (x.detach().double().softmax(1) - torch.nn.functional.one_hot(y.long(), 500))
+    best = x.argmax(1, keepdim=True)
+    want = hard.gather(1, best) + soft
+    assert ((g.gather(1, best) - want).abs() <= 2.0 ** -20 * want.abs()).all()
+    # tau^2 times differences of logits / tau of at most 4 / tau
+    assert ((loss - 0.5 * alone).abs() <= 0.5 * 8 * 4e-6 + 2.0 ** -20 * alone).all()
