@@ -247,11 +247,55 @@ def qk_norm_rope(qkv, wq, wk, cos, sin, T, H, kv_heads=None, eps=1e-5, il=False)
     return _QKNormRope.apply(*args) if _needs_grad(qkv, wq, wk) else _qk_heads(*args)
 
 
+def _extent(t: torch.Tensor) -> int:
+    """Bytes from the first element of ``t`` to behind its last."""
+    if t.is_contiguous():
+        return t.nbytes
+    return (1 + sum([(m - 1) * s for m, s in zip(t.shape, t.stride())])) * t.element_size()
+
+
+def _meet(off: int, dims) -> bool:
+    """Whether ``off`` is a difference of two places of a layout: (stride, size) from the largest stride
+    on, each larger than what the strides behind it reach."""
+    if not dims:
+        return off == 0
+    (s, m), rest = dims[0], dims[1:]
+    return any(abs(i) < m and _meet(off - i * s, rest) for i in (off // s, off // s + 1))
+
+
+def _check_written(kcache, vcache, qkv) -> None:
+    """Both caches are written while qkv is read: no place of theirs may be another's."""
+    k0, v0, x0 = kcache.data_ptr(), vcache.data_ptr(), qkv.data_ptr()
+    if kcache.is_contiguous() and vcache.is_contiguous() and qkv.is_contiguous():
+        n = kcache.nbytes                        # the cheap way: three dense tensors, one behind another
+        x1 = x0 + qkv.nbytes
+        if (k0 + n <= v0 or v0 + n <= k0) and (k0 + n <= x0 or x1 <= k0) and (v0 + n <= x0 or x1 <= v0):
+            return
+    k1, v1, x1 = k0 + _extent(kcache), v0 + _extent(vcache), x0 + _extent(qkv)
+    if not kcache.numel():
+        return
+    for c in (kcache, vcache):
+        if not c.is_contiguous():
+            reach = 0
+            for s, m in sorted([(s, m) for s, m in zip(c.stride(), c.shape) if m > 1]):
+                if s <= reach:
+                    raise ValueError("the caches are written: no expanded tensors, none that overlap themselves")
+                reach += (m - 1) * s
+    if k0 < v1 and v0 < k1:                      # apart, or one between the other's rows in one layout
+        off, rest = divmod(v0 - k0, kcache.element_size())
+        layout = [[(s, m) for s, m in zip(c.stride(), c.shape) if m > 1] for c in (kcache, vcache)]
+        if rest or layout[0] != layout[1] or _meet(off, sorted(layout[0], reverse=True)):
+            raise ValueError("the caches are written: not one for both, and no overlapping ones")
+    if (k0 < x1 and x0 < k1) or (v0 < x1 and x0 < v1):
+        raise ValueError("the caches are written while qkv is read: not in one another's memory")
+
+
 def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=1e-5, il=False):
     """:func:`qk_norm_rope` of the next ``T`` tokens of every sequence: sequence b's stand at
     positions ``start[b] ... start[b] + T - 1`` (int32 ``[B']``, on the device), their keys and
     values are written into ``kcache``, ``vcache`` ``[B', KV, capacity, D]`` at these positions
     (nothing else of the caches is touched), and their queries ``[B', H, T, D]`` are returned.
+    The caches may lie side by side in one tensor, but overlap neither each other nor ``qkv``.
     A token whose position lies outside the cache or the tables is not written, its query is 0.
     No gradients."""
     if kcache.dim() != 4 or kcache.shape != vcache.shape:
@@ -263,17 +307,15 @@ def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=
         raise ValueError(f"the caches are {tuple(kcache.shape)}: {n} sequences of heads of {D}")
     if kcache.dtype != qkv.dtype or vcache.dtype != qkv.dtype:
         raise ValueError("the caches must be of qkv's type")
-    ks, vs = kcache.stride(), vcache.stride()
-    if (0 in ks + vs and any(s == 0 and m > 1 for s, m in zip(ks + vs, kcache.shape * 2))) or \
-            (kcache.numel() and kcache.data_ptr() == vcache.data_ptr()):
-        raise ValueError("the caches are written: no expanded tensors, and not one for both")
+    _check_written(kcache, vcache, qkv)
     _same(qkv, "kcache vcache start", kcache, vcache, start)
     _int32("start", start, n)
     if not _hip(qkv, "qk_norm_rope"):
         return _cached_ref(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps, il)
     _check_kernel("qk_norm_rope_cached", qkv, D)
     _no_tangents("qk_norm_rope_cached", qkv, wq, wk, cos, sin, kcache, vcache)
-    for name, c, s in (("kcache", kcache, ks), ("vcache", vcache, vs)):
+    for name, c in (("kcache", kcache), ("vcache", vcache)):
+        s = c.stride()
         if s[3] != 1 or c.data_ptr() % 16 or (s[0] | s[1] | s[2]) % 8:
             raise ValueError(f"{name} needs contiguous rows at multiples of 16 bytes: it is written "
                              "in place")

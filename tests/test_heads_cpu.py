@@ -365,3 +365,53 @@ def test_references_have_forward_mode_derivatives():
     h = 1e-6
     ends = [heads.window_attention(q + s * d, q, q, 2, 1) for s in (h, -h)]
     torch.testing.assert_close(got, (ends[0] - ends[1]) / (2 * h), rtol=1e-6, atol=1e-8)
+
+
+# ------------------------------------------------------------------------------- memory of the caches
+def _cached_call(kc, vc, qkv=None):
+    n, KV, _, D = kc.shape
+    rows = torch.ones(n, 3 * KV * D) if qkv is None else qkv
+    return heads.qk_norm_rope_cached(rows, torch.ones(1, D), torch.ones(1, D), *heads.rope_tables(4, D), 1, KV, kc, vc,
+                                     torch.zeros(n, dtype=torch.int32))
+
+
+def _overlapping():
+    flat = torch.zeros(4096)
+    yield "shifted", flat[:128].view(2, 2, 4, 8), flat[8:136].view(2, 2, 4, 8)
+    yield "one element", flat[:128].view(2, 2, 4, 8), flat[127:255].view(2, 2, 4, 8)
+    wide = torch.zeros(2, 2, 4, 16)
+    yield "columns", wide[..., :8], wide[..., 7:15]
+    yield "another order", flat[:128].view(2, 2, 4, 8), flat[64:192].view(2, 4, 2, 8).transpose(1, 2)
+    yield "heads of one cache", flat.as_strided((2, 2, 4, 8), (64, 16, 8, 1)), flat[2048:2176].view(2, 2, 4, 8)
+    yield "sequences of the other", flat[2048:2176].view(2, 2, 4, 8), flat.as_strided((2, 2, 4, 8), (24, 32, 8, 1))
+
+
+@pytest.mark.parametrize("name,kc,vc", list(_overlapping()))
+def test_overlapping_caches_are_refused(name, kc, vc):
+    """Both are written at once: where they share memory the last write wins."""
+    with pytest.raises(ValueError, match="written"):
+        _cached_call(kc, vc)
+
+
+def test_caches_over_the_activation_are_refused():
+    flat = torch.ones(512)
+    for at in (0, 95):
+        with pytest.raises(ValueError, match="written"):
+            _cached_call(flat[at:at + 128].view(2, 2, 4, 8), torch.zeros(2, 2, 4, 8), flat[:96].view(2, 48))
+        with pytest.raises(ValueError, match="written"):
+            _cached_call(torch.zeros(2, 2, 4, 8), flat[at:at + 128].view(2, 2, 4, 8), flat[:96].view(2, 48))
+    _cached_call(flat[96:224].view(2, 2, 4, 8), flat[224:352].view(2, 2, 4, 8), flat[:96].view(2, 48))
+
+
+@pytest.mark.parametrize("layout", ["halves", "columns", "by sequence", "by head", "by position", "transposed"])
+def test_caches_side_by_side_in_one_tensor_are_taken(layout):
+    shape, pick = {
+        "halves": ((2, 2, 2, 4, 8), lambda t: (t[0], t[1])), "columns": ((2, 2, 4, 16), lambda t: (t[..., :8], t[..., 8:])),
+        "by sequence": ((2, 2, 2, 4, 8), lambda t: (t[:, 0], t[:, 1])),
+        "by head": ((2, 4, 4, 8), lambda t: (t[:, ::2], t[:, 1::2])),
+        "by position": ((2, 2, 8, 8), lambda t: (t[:, :, :4], t[:, :, 4:])),
+        "transposed": ((2, 4, 4, 8), lambda t: (t[:, :, :2].transpose(1, 2), t[:, :, 2:].transpose(1, 2)))}[layout]
+    kc, vc = pick(torch.zeros(shape))
+    apart = [torch.zeros(2, 2, 4, 8) for _ in "kv"]
+    assert torch.equal(_cached_call(kc, vc), _cached_call(*apart))
+    assert torch.equal(kc, apart[0]) and torch.equal(vc, apart[1]) and kc.any() and vc.any()
