@@ -72,6 +72,8 @@ class _Distill(torch.autograd.Function):
                                                       device=logits.device)
             loss = _launch(logits, labels, top, index, tau, alpha, rows_per_trial, scale, None, grad,
                            True)
+            if inplace:                # (who else kept the logits for a backward has to know)
+                torch.autograd.graph.increment_version(logits)
             ctx.save_for_backward(grad)
             return loss
         mixed = [t for t in (tau, alpha) if torch.is_tensor(t)]
@@ -128,7 +130,8 @@ def distill_loss(logits, labels, top_values, top_index, rows_per_trial, temperat
     ``grad_scale`` multiplies the gradient (``1 / rows_per_trial``: mean-loss gradients).
     ``unit_weights=True`` promises that the result is differentiated through ``loss.sum()`` only:
     the gradient comes out of the forward pass (one read of the logits, one write) and takes the
-    logits' place with ``inplace=True``.  Without it the backward reads the logits again."""
+    logits' place with ``inplace=True`` (a write in place to autograd: an operation that kept the
+    logits for its own backward refuses it).  Without it the backward reads the logits again."""
     if logits.dim() != 2 or not logits.is_floating_point():
         raise ValueError("logits are [rows, vocabulary]")
     R, V = logits.shape

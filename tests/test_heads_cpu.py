@@ -415,3 +415,27 @@ def test_caches_side_by_side_in_one_tensor_are_taken(layout):
     apart = [torch.zeros(2, 2, 4, 8) for _ in "kv"]
     assert torch.equal(_cached_call(kc, vc), _cached_call(*apart))
     assert torch.equal(kc, apart[0]) and torch.equal(vc, apart[1]) and kc.any() and vc.any()
+
+
+# ------------------------------------------------------------------------------- writes that autograd has to see
+def test_distill_in_place_marks_the_logits_as_written(monkeypatch):
+    """Another operation that kept the logits for its backward says so, as after any write in place."""
+    monkeypatch.setattr(distill, "_hip", lambda t, op="": True)
+    monkeypatch.setattr(distill, "_call", lambda x, name, *args: None)
+    leaf = torch.randn(4, 5, requires_grad=True)
+    y, top, index = torch.zeros(4, dtype=torch.int32), torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32)
+    for inplace in (False, True):
+        h = leaf * 2
+        other = (h * h).sum()
+        loss = distill.distill_loss(h.view(4, 5), y, top, index, 2, unit_weights=True, inplace=inplace)
+        g, = torch.autograd.grad(loss.sum(), h, retain_graph=True)        # (its own backward runs)
+        assert (g.data_ptr() == h.data_ptr()) == inplace
+        if not inplace:
+            torch.autograd.grad(other, leaf)
+            continue
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(other, leaf)
+    with torch.no_grad():                              # without a gradient nothing is written
+        before = h._version
+        distill.distill_loss(h, y, top, index, 2, unit_weights=True, inplace=True)
+        assert h._version == before
