@@ -321,8 +321,10 @@ def qk_norm_rope_cached(qkv, wq, wk, cos, sin, T, H, kcache, vcache, start, eps=
                              "in place")
     if cap == 0 or not len(cos):
         return torch.zeros(n, H, T, D, dtype=qkv.dtype, device=qkv.device)
-    return _qk_fwd(_rows16(qkv), _dense16(wq), _dense16(wk), cos, sin, T, H, KV, float(eps), il,
-                   kcache, vcache, start, cap)
+    q = _qk_fwd(_rows16(qkv), _dense16(wq), _dense16(wk), cos, sin, T, H, KV, float(eps), il, kcache,
+                vcache, start, cap)
+    torch.autograd.graph.increment_version((kcache, vcache))     # written behind torch's back
+    return q
 
 
 @torch.no_grad()

@@ -439,3 +439,24 @@ def test_distill_in_place_marks_the_logits_as_written(monkeypatch):
         before = h._version
         distill.distill_loss(h, y, top, index, 2, unit_weights=True, inplace=True)
         assert h._version == before
+
+
+@pytest.mark.parametrize("kernel", [False, True])
+def test_cached_heads_mark_the_caches_as_written(kernel, monkeypatch):
+    """Attention over the caches keeps them for its backward, which a later write into them would falsify."""
+    if kernel:
+        monkeypatch.setattr(heads, "_hip", lambda t, op="": True)
+        monkeypatch.setattr(heads, "_call", lambda *args: None)
+    bf, w = torch.bfloat16, torch.ones(1, 64, dtype=torch.bfloat16)
+    kc, vc = (torch.randn(2, 1, 4, 64).to(bf) for _ in "kv")
+    q = torch.randn(2, 1, 1, 64).to(bf).requires_grad_(True)
+    start = torch.full((2,), 2, dtype=torch.int32)
+    if kernel:
+        o = heads._WindowAttention.apply(q, kc, vc, 9, 0, 0.125, start, 3, None)
+    else:
+        o = (q * kc).sum() + (q * vc).sum()
+    before = kc._version, vc._version
+    heads.qk_norm_rope_cached(torch.ones(2, 192, dtype=bf), w, w, *heads.rope_tables(4, 64), 1, 1, kc, vc, start)
+    assert kc._version > before[0] and vc._version > before[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(o.float().sum(), q)
