@@ -154,3 +154,51 @@ def test_task_builds_them():
         pop.set_member(s, task.member_config({"/lr": 1e-3, "/steps": 1}, s))
     pop.train_step(*data.batch(0))
     assert np.isfinite(pop.train_loss()[0])
+
+
+def _with_weights(pop, std, seed=1):
+    """Matrices of N(0, std), norms of N(1, 0.2): weights with which every part counts."""
+    rng = torch.Generator().manual_seed(seed)
+    with torch.no_grad():
+        for name, w in pop.W.items():
+            w.copy_(torch.randn(w.shape, generator=rng) * (0.2 if "norm" in name else std) + ("norm" in name))
+    return pop
+
+
+@pytest.mark.parametrize("options", [FULL, dict(window=20, sinks=3)])
+@pytest.mark.parametrize("distill", [None, (0.4, 2.0)])
+def test_gradients_have_the_slope_s_size_and_direction(options, distill):
+    """Along a gradient the loss rises by its norm: no other direction is as steep, and a gradient that is
+    scaled or lacks a part is told by it.
+
+    The loss, of at most 12 for 512 tokens, passes some 32-bit pieces: 16 roundings of it are 1.2e-5 at
+    most, over 2 h 6e-4.  The third derivative's share, h^2 of the slope's size times what a step of 1
+    changes of it (some tens), is under 1 %."""
+    pop = _with_weights(_in_64_bits(_population(distill, **options)), 0.15)
+    x, y = SyntheticLM(512, 64, 2, n_tokens=1 << 12, teacher_top=5 if distill else 0).batch(0)
+    loss = lambda: pop._loss(x, y, True).sum() / x.numel()  # noqa: E731
+    pop._loss(x, y, True).sum().backward()     # (gradients are those of the mean over a trial's rows)
+    h = 1e-2
+    for name, w in pop.W.items():
+        size = w.grad.norm().item()
+        assert size > 0.03, name               # (well over what the tolerance leaves open)
+        with torch.no_grad():
+            d = h * w.grad / size
+            ends = [(w.add_(s * d), loss().item(), w.sub_(s * d))[1] for s in (1, -1)]
+        slope = (ends[0] - ends[1]) / (2 * h)
+        assert abs(slope - size) <= 0.01 * size + 16 * 12 * 2.0 ** -24 / (2 * h), (name, slope, size)
+
+
+def test_a_window_over_all_tokens_is_plain_attention_and_a_shorter_one_is_not():
+    """Rows of logits, in 64 bits but for the plain attention's 32: 2^-24 times some hundred operations."""
+    x = SyntheticLM(512, 64, 2, n_tokens=1 << 12).batch(0)[0]
+
+    def logits(**options):
+        pop = _with_weights(_in_64_bits(_population(**options)), 0.15)
+        with torch.no_grad():
+            return pop._logits(pop._expand(x, torch.int32), pop._attention)
+    plain = logits()
+    off = {w: ((logits(window=w, sinks=s) - plain).norm() / plain.norm()).item()
+           for w, s in ((64, 1), (63, 0), (5, 0))}
+    assert off[64] <= 500 * 2.0 ** -24
+    assert off[63] > 20 * 500 * 2.0 ** -24 and off[5] > 0.1, off
