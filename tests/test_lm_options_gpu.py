@@ -178,3 +178,47 @@ def test_greedy_continuations():
         chosen = last.gather(-1, got[:, :, step:step + 1].long())[..., 0]
         assert (top - chosen <= 2 * 40 * U * last.abs().amax()).all()
         tok = torch.cat([tok, got[:, :, step:step + 1]], -1)
+
+
+def _with_weights(pop, std, seed=1):
+    """Matrices of N(0, std), norms of N(1, 0.2), as 16-bit values, the same on either device."""
+    rng = torch.Generator().manual_seed(seed)
+    with torch.no_grad():
+        for name, w in pop.W.items():
+            t = torch.randn(w.shape, generator=rng) * (0.2 if "norm" in name else std) + ("norm" in name)
+            w.copy_(t.to(BF))
+    return pop
+
+
+@pytest.mark.parametrize("options,distilled,wrong", [
+    (FULL, (0.4, 2.0), [dict(window=19), dict(window=21), dict(sinks=2), dict(sinks=4)]),
+    (dict(window=20, sinks=3), None, [dict(window=19), dict(sinks=2)]),
+    (dict(n_heads=1, qk_norm=True), (1.0, 1.0), [dict(window=48)])])
+def test_population_gradients_tell_a_token_more_or_less(options, distilled, wrong):
+    """Loss and gradients of the population against the model in 64 bits with the same 16-bit weights, and
+    how far those of a window or sinks one token off are (where all 64 are seen: of a window of 48).
+
+    About 40 tensors between a weight and the loss are rounded once, each value by at most U of it and, over
+    values, by U / sqrt(3) at the root of the mean square; independent, they add up to sqrt(40 / 3) U =
+    1.4 %.  Two layers' norms and softmaxes pass errors on about as they are: 12 U = 4.7 % is three times
+    that.  The mean loss is such a sum over 512 tokens, each off by 1.4 % of its logits' size at most."""
+    limit = 12 * U
+    x, y = _data(distilled).batch(0)
+    host = tuple(t.cpu() for t in y) if isinstance(y, tuple) else y.cpu()
+    gpu = _with_weights(_population(options, distilled, graph=False), 0.06)
+    loss = gpu._loss(x, y, True)
+    loss.backward(torch.ones_like(loss))
+
+    def exact(**changes):
+        pop = _population(dict(options, **changes), distilled, "cpu")
+        pop.W = {k: w.detach().double().requires_grad_(True) for k, w in _with_weights(pop, 0.06).W.items()}
+        loss = pop._loss(x.cpu(), host, True)
+        loss.sum().backward()
+        return loss.detach(), {k: w.grad for k, w in pop.W.items()}
+    want, grads = exact()
+    assert ((loss.detach().cpu() - want).abs() <= limit / 3 * want.abs()).all()
+    far = {k: _off(gpu.W[k].grad.cpu(), g) for k, g in grads.items()}
+    assert max(far.values()) <= limit, far
+    for changes in wrong:
+        other = exact(**changes)[1]
+        assert max(_off(other[k], g) for k, g in grads.items()) > 2 * limit, changes
