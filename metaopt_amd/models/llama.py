@@ -197,9 +197,9 @@ class PopulationLM(FlatPopulation):
         return distill_loss(logits, labels, values, index, rpt, self.temperature, self.alpha,
                             grad_scale=1.0 / rpt, unit_weights=True, inplace=True)
 
-    def _logits(self, tok: torch.Tensor, attend):
-        """Rows of logits of the tokens ``[P, sequences, T]``; ``attend(l, h, T)``: layer l's
-        attention output of the normalised rows h."""
+    def _logits(self, tok: torch.Tensor, attend, last: bool = False):
+        """Rows of logits of the tokens ``[P, sequences, T]`` (``last``: of each sequence's last
+        token); ``attend(l, h, T)``: layer l's attention output of the normalised rows h."""
         c, P, W = self.cfg, self.capacity, self.W
         R, T, d = tok.numel(), tok.shape[-1], c.d_model
         rpt = R // P
@@ -216,7 +216,8 @@ class PopulationLM(FlatPopulation):
             y = ops.swiglu_mlp(h.view(P, rpt, d), W[f"l{l}.wgu"], W[f"l{l}.wdown"])
             nxt = W[f"l{l + 1}.attn_norm"] if l + 1 < c.n_layers else W["final_norm"]
             x, h = ops.add_rmsnorm(x, y.view(R, d), nxt, rpt, c.norm_eps)
-        return _lin(h.view(P, rpt, d), W["head"]).view(R, c.vocab)
+        h = h.view(P, -1, T, d)[:, :, -1] if last else h.view(P, rpt, d)
+        return _lin(h, W["head"]).view(-1, c.vocab)
 
     def _attention(self, l, h, T):
         c, W = self.cfg, self.W
@@ -256,9 +257,9 @@ class PopulationLM(FlatPopulation):
             return heads.window_attention(q, kcache[l], vcache[l], c.window, c.sinks, start=start)
         out, tok = [], self._expand(tok, torch.int32)
         for _ in range(steps):
-            logits = self._logits(tok, attend).view(P, n, -1, c.vocab)
+            logits = self._logits(tok, attend, last=True).view(P, n, 1, c.vocab)
             start += tok.shape[-1]
-            tok = logits[:, :, -1:].argmax(-1).to(torch.int32)
+            tok = logits.argmax(-1).to(torch.int32)
             out.append(tok)
         return torch.cat(out, -1)
 

@@ -202,3 +202,19 @@ def test_a_window_over_all_tokens_is_plain_attention_and_a_shorter_one_is_not():
            for w, s in ((64, 1), (63, 0), (5, 0))}
     assert off[64] <= 500 * 2.0 ** -24
     assert off[63] > 20 * 500 * 2.0 ** -24 and off[5] > 0.1, off
+
+
+def test_greedy_forms_logits_of_last_tokens_only(monkeypatch):
+    """A prompt's other rows, vocabulary wide, are the largest tensors there would be."""
+    from metaopt_amd.models import llama
+    pop = _population(**FULL)
+    prompt = SyntheticLM(512, 64, 3, n_tokens=1 << 12).batch(0)[0][:, :30]
+    rows, lin = [], llama._lin
+
+    def watched(x, w):
+        if w is pop.W["head"]:
+            rows.append(x.shape[1])
+        return lin(x, w)
+    monkeypatch.setattr(llama, "_lin", watched)
+    pop.greedy(prompt, 4)
+    assert rows == [3] * 4, rows
