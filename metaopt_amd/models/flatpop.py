@@ -530,7 +530,7 @@ class FlatPopulation:
             if self.v.numel():
                 self.v[sl] = state["v32"][o:o + n]
             o += n
-        if "aux" in state and self.n_aux:
+        if self.n_aux and len(state.get("aux", ())):     # (a state without any leaves the slot's)
             self._set_aux(slot, state["aux"])
         cfg = MemberConfig(**state["config"])
         self.members[slot] = cfg

@@ -134,7 +134,8 @@ class PopulationLM(FlatPopulation):
         """``distill``: (alpha, temperature) of :func:`~metaopt_amd.ops.distill.distill_loss` --
         training batches are then (tokens, (labels, teacher's top logits, their indices)), as
         ``SyntheticLM(teacher_top=...)`` gives them.  ``self.alpha`` and ``self.temperature`` hold
-        one value a trial and may be written in place between steps."""
+        one value a trial and may be written in place between steps; they go with the trial's
+        weights into checkpoints and copies, and a new trial (``set_member``) has those given here."""
         if moment_dtype is not None:       # AdamW first-moment storage (mopt sweep --dtype)
             self.moment_dtype = moment_dtype
         self.cfg = PRESETS[config] if isinstance(config, str) else config
@@ -148,18 +149,28 @@ class PopulationLM(FlatPopulation):
         self.batch_size = int(batch_size)          # sequences per trial per step
         self.eval_batch = int(eval_batch or batch_size)
         self.tokens_per_step = self.batch_size * c.seq_len
+        self.distill = distill is not None
+        if self.distill:
+            self._first_mix = alpha, temperature = tuple(float(x) for x in distill)
+            if not (0.0 <= alpha <= 1.0 and temperature > 0.0):
+                raise ValueError(f"distill {distill}: (alpha in [0, 1], temperature > 0)")
         super().__init__(capacity, device=device, max_grad_norm=max_grad_norm,
                          use_graph=use_graph)
         self.cos, self.sin = (ops.rope_tables(c.seq_len, c.rope_base, device=self.device)
                               if not c.qk_norm else
                               heads.rope_tables(c.seq_len, c.head_dim, c.rope_base, self.device))
-        self.distill = distill is not None
         if self.distill:
-            alpha, temperature = (float(x) for x in distill)
-            if not (0.0 <= alpha <= 1.0 and temperature > 0.0):
-                raise ValueError(f"distill {distill}: (alpha in [0, 1], temperature > 0)")
-            full = lambda x: torch.full((self.capacity,), x, device=self.device)  # noqa: E731
-            self.alpha, self.temperature = full(alpha), full(temperature)
+            self.alpha, self.temperature = self.A["mix"][:, 0], self.A["mix"][:, 1]
+            for slot in range(self.capacity):
+                self.init_aux(slot)
+
+    def aux_specs(self):
+        return [("mix", 4)] if self.distill else []      # alpha, temperature (copied 4 values at a time)
+
+    def init_aux(self, slot: int) -> None:
+        if self.distill:
+            for i, x in enumerate(self._first_mix):
+                self.A["mix"][slot, i] = x
 
     def param_specs(self):
         return param_specs(self.cfg)
@@ -194,8 +205,9 @@ class PopulationLM(FlatPopulation):
             raise ValueError("distillation takes batches (tokens, (labels, top values, top indices))")
         values, index = (self._expand(t, kind).reshape(P * rpt, -1)
                          for t, kind in zip(top, (None, torch.int32)))
-        return distill_loss(logits, labels, values, index, rpt, self.temperature, self.alpha,
-                            grad_scale=1.0 / rpt, unit_weights=True, inplace=True)
+        return distill_loss(logits, labels, values, index, rpt, self.temperature.contiguous(),
+                            self.alpha.contiguous(), grad_scale=1.0 / rpt, unit_weights=True,
+                            inplace=True)
 
     def _logits(self, tok: torch.Tensor, attend, last: bool = False):
         """Rows of logits of the tokens ``[P, sequences, T]`` (``last``: of each sequence's last

@@ -218,3 +218,41 @@ def test_greedy_forms_logits_of_last_tokens_only(monkeypatch):
     monkeypatch.setattr(llama, "_lin", watched)
     pop.greedy(prompt, 4)
     assert rows == [3] * 4, rows
+
+
+def test_a_trial_s_mix_goes_where_its_weights_go():
+    """alpha and temperature of a trial are in its checkpoints, in what is sent to another rank and in copies
+    between slots; a new trial has those that the population was built with."""
+    pop = _population((0.4, 2.0), **FULL)
+    pop.alloc_ckpt_pool(2)
+    mix = lambda s, p=pop: (p.alpha[s].item(), p.temperature[s].item())  # noqa: E731
+    first = (pytest.approx(0.4), 2.0)
+    assert [mix(0), mix(1)] == [first] * 2
+    pop.alpha[0], pop.temperature[0] = 0.75, 3.5
+    meta, = pop.save_states([(0, 1)])
+    sent = pop.unpack_state(pop.pack_state(pop.pool_state(meta)).clone())
+    state = pop.slot_state(0)
+    pop.set_member(0, MemberConfig(width=128, lr=1e-3, seed=9))
+    assert mix(0) == first
+    pop.load_states([(1, meta)])
+    assert [mix(0), mix(1)] == [first, (0.75, 3.5)]
+    pop.load_slot_state(0, state)
+    assert mix(0) == (0.75, 3.5)
+    pop.set_member(1, MemberConfig(width=128, lr=1e-3, seed=10))
+    pop.copy_member(0, 1)
+    assert mix(1) == (0.75, 3.5)
+    other = _population((0.1, 1.0), **FULL)
+    other.load_slot_state(0, sent)
+    assert mix(0, other) == (0.75, 3.5) and mix(1, other) == (pytest.approx(0.1), 1.0)
+    tensors = pop.c4_send_tensors(meta)
+    got = other._c4_header()
+    got.copy_(tensors[1])
+    other.alloc_ckpt_pool(1)
+    other._ck[0].copy_(tensors[0])
+    other.load_states([(1, other.c4_finish(0, [other._ck[0], got]))])
+    assert mix(1, other) == (0.75, 3.5)
+    # a state of a population without a mix (or from before it was kept) leaves the slot's
+    plain = _population(None, **FULL)
+    assert plain.n_aux == 0
+    other.load_slot_state(0, plain.slot_state(0))
+    assert mix(0, other) == (0.75, 3.5)

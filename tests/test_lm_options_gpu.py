@@ -222,3 +222,21 @@ def test_population_gradients_tell_a_token_more_or_less(options, distilled, wron
     for changes in wrong:
         other = exact(**changes)[1]
         assert max(_off(other[k], g) for k, g in grads.items()) > 2 * limit, changes
+
+
+def test_a_trial_s_mix_is_in_its_checkpoints():
+    """... and a captured step reads what was loaded."""
+    pops = [_population(FULL, (0.4, 2.0), graph=g, lr=0.0) for g in (True, False)]
+    data, seen = _data(True), []
+    for pop in pops:
+        pop.alloc_ckpt_pool(1)
+        pop.train_step(*data.batch(0))
+        pop.alpha[0], pop.temperature[0] = 0.75, 3.5
+        meta, = pop.save_states([(0, 0)])
+        pop.set_member(0, MemberConfig(width=128, lr=0.0, seed=7, beta2=0.95))
+        assert (pop.alpha[0].item(), pop.temperature[0].item()) == (torch.tensor(0.4).item(), 2.0)
+        pop.load_states([(1, meta)])
+        assert (pop.alpha[1].item(), pop.temperature[1].item()) == (0.75, 3.5)
+        pop.train_step(*data.batch(0))
+        seen.append(pop.train_loss())
+    assert np.array_equal(*seen) and seen[0][0] != seen[0][1]
