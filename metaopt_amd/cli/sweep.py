@@ -54,6 +54,9 @@ def add_subparser(parser):
     g.add_argument("--dtype", default="bf16", choices=["bf16", "fp32"],
                    help="optimizer-state storage precision (compute: bf16 MFMA, fp32 accum)")
     g.add_argument("--population", type=int, default=None, help="trials per GPU")
+    g.add_argument("--task-options", default=None, metavar="JSON",
+                   help="options of the task as a JSON object; LM tasks: model (qk_norm, kv_heads, "
+                        "window, sinks, ...), distill ([alpha, temperature]), teacher_top")
     g.add_argument("--max-trials", type=int, default=None)
     g.add_argument("--steps", type=int, default=100000, help="max population steps")
     g.add_argument("--sync-every", type=int, default=32)
@@ -157,8 +160,9 @@ def run(args):
     from ..worker.population_sweep import PopulationSweep
     from ..worker.tasks import get
 
-    comm = init_from_env()
     spec = get(args["task"])
+    options = spec.parse_options(args.get("task_options"))
+    comm = init_from_env()
     P = args["population"] or DEFAULT_POPULATION.get(args["task"], 64)
     experiment = None
     priors = None
@@ -169,7 +173,7 @@ def run(args):
     # every rank builds its population for the same (stored) space
     priors = comm.broadcast_object(priors)
     task, pop, data = spec.build(P, comm.device, args["seed"], priors=priors,
-                                 state_dtype=args.get("dtype", "bf16"))
+                                 state_dtype=args.get("dtype", "bf16"), **options)
     events = watchdog = None
     if args.get("event_log"):
         from ..utils.events import EventLog

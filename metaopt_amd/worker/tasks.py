@@ -33,6 +33,7 @@ class TaskSpec:
     tunable: Tuple[str, ...] = ()
     required: Tuple[str, ...] = ("/lr",)       # must be in every space
     needs_fidelity: bool = False               # budgets come from the /steps fidelity only
+    options: Tuple[str, ...] = ()              # arguments of ``build`` a sweep may give (--task-options)
 
     def check_space(self, space) -> None:
         """Refuse a user space this task cannot train: unknown names, missing required ones,
@@ -50,6 +51,23 @@ class TaskSpec:
             raise ValueError(f"the fidelity dimension must be /steps (optimizer steps), got {fids}")
         if self.needs_fidelity and not fids:
             raise ValueError("this task needs a /steps fidelity (its trials' budgets)")
+
+
+    def parse_options(self, text) -> dict:
+        """The arguments of ``build`` in the JSON object ``text`` (None: none)."""
+        if not text:
+            return {}
+        import json
+        try:
+            options = json.loads(text)
+        except json.JSONDecodeError as exc:
+            raise ValueError(f"task options are a JSON object: {exc}") from None
+        if not isinstance(options, dict):
+            raise ValueError("task options are a JSON object")
+        unknown = sorted(set(options) - set(self.options))
+        if unknown:
+            raise ValueError(f"task option(s) {unknown} are not known here; there are: {sorted(self.options)}")
+        return options
 
 
 def _max_width(priors, default):
@@ -127,6 +145,9 @@ def _lm(population, device, seed, preset="llama-125m", batch_size=8, seq_len=512
     import dataclasses
     import torch
     from ..models.llama import PRESETS, LM_PBT_PRIORS, LMSweepTask, PopulationLM, SyntheticLM
+    known = {f.name for f in dataclasses.fields(PRESETS[preset])}
+    if set(model or ()) - known:
+        raise ValueError(f"model option(s) {sorted(set(model) - known)}: there are {sorted(known)}")
     cfg = dataclasses.replace(PRESETS[preset], **(model or {}))
     task = LMSweepTask(priors=dict(priors or LM_PBT_PRIORS), d_model=cfg.d_model)
     pop = PopulationLM(population, cfg, batch_size=batch_size, seq_len=seq_len, distill=distill,
@@ -169,7 +190,7 @@ TASKS: Dict[str, TaskSpec] = {
                          "/steps": "fidelity(200, 2000, 2)"},
                         _pbt(200), _lm, 8 * 512, "tokens/s", ckpt_factor=2.0,
                         tunable=("/lr", "/weight_decay", "/beta1", "/steps"),
-                        needs_fidelity=True),
+                        needs_fidelity=True, options=("model", "distill", "teacher_top")),
     "lm-tiny": TaskSpec({"/lr": "loguniform(1e-4, 3e-3)",
                          "/weight_decay": "loguniform(1e-3, 0.3)", "/beta1": "uniform(0.8, 0.95)",
                          "/steps": "fidelity(200, 2000, 2)"},
@@ -177,7 +198,7 @@ TASKS: Dict[str, TaskSpec] = {
                                                              seq_len=256, **kw),
                         8 * 256, "tokens/s", ckpt_factor=2.0,
                         tunable=("/lr", "/weight_decay", "/beta1", "/steps"),
-                        needs_fidelity=True),
+                        needs_fidelity=True, options=("model", "distill", "teacher_top")),
 }
 
 
