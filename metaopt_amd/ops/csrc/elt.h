@@ -14,6 +14,14 @@ struct Bf16 {
   static constexpr int kShift = 0;
   static __device__ __forceinline__ float up(uint32_t h) { return bf2f((bf16_t)h); }
   static __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack2bf(a, b); }
+  // (a, b) minus the halves of p: a's difference is p . (-1, 0) + a, one instruction with no unpacking
+  static __device__ __forceinline__ f32x2_t less2(float a, float b, uint32_t p) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    uint32_t lo = 0xBF80u, hi = 0xBF800000u;             // (-1, 0), (0, -1)
+    asm("" : "+s"(lo), "+s"(hi));                        // (in registers, not as an f32 constant)
+    return f32x2_t{__builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, p), __builtin_bit_cast(pair, lo), a, false),
+                   __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, p), __builtin_bit_cast(pair, hi), b, false)};
+  }
   static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -34,6 +42,10 @@ struct Fp16 {
   }
   static __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, f16x2_t));
+  }
+  static __device__ __forceinline__ f32x2_t less2(float a, float b, uint32_t p) {
+    const f16x2_t h = __builtin_bit_cast(f16x2_t, p);
+    return f32x2_t{fmaf((float)h[0], -1.f, a), fmaf((float)h[1], -1.f, b)};
   }
   static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),

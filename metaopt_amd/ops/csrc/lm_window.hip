@@ -12,7 +12,7 @@
 // Scores are formed transposed (S^T = K Q^T, a lane is one query) with the K rows fed in an order
 // that exchanges bits 2 and 3 of the row: register r of lane half h is then key
 // 16 (r >> 3) + 8 h + (r & 7), so registers 8 s ... 8 s + 7 are, converted and packed, the B
-// operand of step s of the product with V -- P never leaves its lane.  V^T is read with the
+// operands (two: see split8) of step s of the product with V -- P never leaves its lane.  V^T is read with the
 // transposing LDS read.  dK / dV do the same with queries in the place of keys.
 #include "elt.h"
 
@@ -96,11 +96,33 @@ struct Place {
   }
 };
 
+// Probabilities and score gradients, held in 32 bits, enter their products as two 16-bit pieces: rounded,
+// and what that rounding left off.  One piece alone made o, dq, dk and dv up to 1.45 times as far from 64
+// bits as outputs that are only rounded in the end; with two they are as near as these.  The price is a
+// product more for each of P V, dS K, P^T dO and dS^T Q: forward 51 -> 64 us (4 x 12 heads of 64, 4096 tokens,
+// window 512), 8192 tokens of 16 / 4 heads of 128, window 1024: 105 -> 131, dQ 144 -> 172, dK / dV 189 -> 246;
+// a single token over a cache 15.0 -> 15.1, memory bounds that.
+struct Two {
+  u32x4 hi, lo;
+};
+template <class E>
+__device__ __forceinline__ Two split8(float a, float b, float c, float d, float e, float f, float g, float h) {
+  Two t;
+  t.hi = u32x4{E::pack2(a, b), E::pack2(c, d), E::pack2(e, f), E::pack2(g, h)};
+  const f32x2_t r0 = E::less2(a, b, t.hi[0]), r1 = E::less2(c, d, t.hi[1]);
+  const f32x2_t r2 = E::less2(e, f, t.hi[2]), r3 = E::less2(g, h, t.hi[3]);
+  t.lo = u32x4{E::pack2(r0[0], r0[1]), E::pack2(r1[0], r1[1]), E::pack2(r2[0], r2[1]), E::pack2(r3[0], r3[1])};
+  return t;
+}
 // registers 8 s ... 8 s + 7 of an accumulator as the B operand of step s
 template <class E>
-__device__ __forceinline__ u32x4 pack(const f32x16& x, int s) {
-  return u32x4{E::pack2(x[8 * s], x[8 * s + 1]), E::pack2(x[8 * s + 2], x[8 * s + 3]),
-               E::pack2(x[8 * s + 4], x[8 * s + 5]), E::pack2(x[8 * s + 6], x[8 * s + 7])};
+__device__ __forceinline__ Two pack(const f32x16& x, int s) {
+  return split8<E>(x[8 * s], x[8 * s + 1], x[8 * s + 2], x[8 * s + 3], x[8 * s + 4], x[8 * s + 5], x[8 * s + 6],
+                   x[8 * s + 7]);
+}
+template <class E>
+__device__ __forceinline__ f32x16 mfma_both(const u32x4& a, const Two& b, f32x16 c) {
+  return E::mfma32(a, b.lo, E::mfma32(a, b.hi, c));
 }
 // the key (query) within a 32-row group that register r of this lane holds
 __device__ __forceinline__ int row_of(int r, int lane) {
@@ -395,10 +417,10 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
         l += part;
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          const u32x4 p = pack<E>(x, st);
+          const Two p = pack<E>(x, st);
 #pragma unroll
           for (int dn = 0; dn < DN; ++dn)
-            acc[dn] = E::mfma32(at.frag_t(Vs + sub * 64 * D, 16 * st, dn), p, acc[dn]);
+            acc[dn] = mfma_both<E>(at.frag_t(Vs + sub * 64 * D, 16 * st, dn), p, acc[dn]);
         }
       };
 #pragma unroll
@@ -516,10 +538,10 @@ __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, 
       auto add = [&](const f32x16& x, int sub) {
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          const u32x4 p = pack<E>(x, st);
+          const Two p = pack<E>(x, st);
 #pragma unroll
           for (int dn = 0; dn < DN; ++dn)
-            acc[dn] = E::mfma32(at.frag_t(Ks + sub * 64 * D, 16 * st, dn), p, acc[dn]);
+            acc[dn] = mfma_both<E>(at.frag_t(Ks + sub * 64 * D, 16 * st, dn), p, acc[dn]);
         }
       };
 #pragma unroll
@@ -724,15 +746,15 @@ struct Dkv {
     }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
-      const u32x4 p = pack<E>(x, st);
+      const Two p = pack<E>(x, st);
 #pragma unroll
-      for (int dn = 0; dn < DN; ++dn) av[dn] = E::mfma32(at.frag_t(Os, 16 * st, dn), p, av[dn]);
+      for (int dn = 0; dn < DN; ++dn) av[dn] = mfma_both<E>(at.frag_t(Os, 16 * st, dn), p, av[dn]);
     }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
-      const u32x4 d = pack<E>(y, st);
+      const Two d = pack<E>(y, st);
 #pragma unroll
-      for (int dn = 0; dn < DN; ++dn) ak[dn] = E::mfma32(at.frag_t(Qs, 16 * st, dn), d, ak[dn]);
+      for (int dn = 0; dn < DN; ++dn) ak[dn] = mfma_both<E>(at.frag_t(Qs, 16 * st, dn), d, ak[dn]);
     }
   }
 
@@ -936,8 +958,7 @@ __global__ __launch_bounds__(NW * 64) void window_step_kernel(WinArgs a, uint16_
           sum += x[h][r];
         }
       l = l * f + sum;
-      const u32x4 p = {E::pack2(x[0][0], x[0][1]), E::pack2(x[0][2], x[0][3]), E::pack2(x[1][0], x[1][1]),
-                       E::pack2(x[1][2], x[1][3])};
+      const Two p = split8<E>(x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const uint16_t* v = vs[wave][buf];
@@ -945,7 +966,8 @@ __global__ __launch_bounds__(NW * 64) void window_step_kernel(WinArgs a, uint16_
         const bf16x8 vf = cat_frag(lds_tr4((const bf16_t*)v + lds_off<D>(r, col)),
                                    lds_tr4((const bf16_t*)v + lds_off<D>(r + 4, col)));
         acc[dt] *= f;
-        acc[dt] = E::mfma16(__builtin_bit_cast(u32x4, vf), p, acc[dt]);
+        acc[dt] = E::mfma16(__builtin_bit_cast(u32x4, vf), p.hi, acc[dt]);
+        acc[dt] = E::mfma16(__builtin_bit_cast(u32x4, vf), p.lo, acc[dt]);
       }
     }
     l = over_groups(l, false);

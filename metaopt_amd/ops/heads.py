@@ -476,7 +476,9 @@ def window_attention(q, k, v, window: Optional[int] = None, sinks: int = 0, scal
     absent, but a value's infinity or NaN reaches the queries whose tiles it shares.
 
     ``scale``: positive (within [1e-30, 1e30]), default ``1 / sqrt(D)``.  Scores and log-sums are
-    kept in 32 bits: beyond 2^16 in size their last bits are felt in the gradients.  Any strides
+    kept in 32 bits: beyond 2^16 in size their last bits are felt in the gradients.  Probabilities and
+    score gradients enter their products as two 16-bit pieces (2^-16 of themselves in bf16, 2^-22 in
+    fp16), so that results are as near as rounded once.  Any strides
     (copied where rows are not contiguous at multiples of 16 bytes).  Differentiable in q, k and v,
     with sums in a fixed order."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:

@@ -456,3 +456,69 @@ def test_window_attention_fp16_large_score_gradients(T):
     """Score gradients past fp16's largest value (65504), whose sums of products over 16 are not."""
     q, k, v, do = _attention_case(1, 2, 2, T, T, 64, FP)
     _check(q, k, (v * 32).half(), (do * 256).half(), 50, 2, scale=0.0625)
+
+
+def _once_rounded(q, k, v, do, window, sinks, scale=None, start=None, lengths=None):
+    """(want, tolerance) of o (and dq, dk, dv) where outputs are rounded to 16 bits and nothing in front of
+    them is: probabilities and score gradients enter their products in two 16-bit pieces, off by u u."""
+    u, (B, H, Tq, D), (KV, Tk) = _u(q.dtype), q.shape, k.shape[1:3]
+    want = [w for w, _ in _attention_oracle(q, k, v, do, window, sinks, start, lengths, scale)]
+    scale = 1 / math.sqrt(D) if scale is None else scale
+    first = torch.full((B,), Tk - Tq, device=DEV) if start is None else start
+    see = heads.window_mask(Tq, Tk, window or Tq + Tk, sinks, first, first + Tq if lengths is None else lengths,
+                            DEV)[:, None, None]
+    some = see.any(-1, keepdim=True)
+    kd, vd = k.detach().double()[:, :, None], v.detach().double()[:, :, None]
+    qd = q.detach().double().view(B, KV, H // KV, Tq, D)
+    s = (qd @ kd.transpose(-1, -2)) * scale
+    p = s.masked_fill(~see, -math.inf).masked_fill(~some, 0).softmax(-1) * see
+    o = p @ vd
+    # a score is D products summed in 32 bits, an exponential is good to 2^-20; the second piece of an fp16
+    # value below 2^-14 is off by 2^-25 of what the row's largest probability (at least 1 / 256) is taken as
+    es = (2 * D * F32 * scale * (qd.abs() @ kd.abs().transpose(-1, -2)) * see).amax() + 2.0 ** -20
+    sub = 2.0 ** -25 if q.dtype == FP else 2.0 ** -126
+    tiny = torch.finfo(q.dtype).tiny * u
+    rough = (u * u + es) * (p @ vd.abs()) + sub * (see.double() @ vd.abs())
+    rows = lambda t: t.reshape(B, H, Tq, D).transpose(1, 2).reshape(B * Tq, H * D)  # noqa: E731
+    tols = [rows(u * o.abs() + rough) + tiny]
+    if do is not None:
+        # (as in the oracle: the log-sum's rounding, added to a score 16 products at a time)
+        es = es + (D / 16 + 2) * F32 * (1.4427 * ((s * see).abs().amax() + math.log(Tk)) + 1)
+        dod = do.double().view(B, Tq, H, D).transpose(1, 2).reshape(B, KV, H // KV, Tq, D)
+        dp, delta = dod @ vd.transpose(-1, -2), (dod * o).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        low = sub * (2.0 ** -12 if q.dtype == FP else 1)
+        dv = (u * u + es) * (p.transpose(-1, -2) @ dod.abs()) + low * (see.double().transpose(-1, -2) @ dod.abs())
+        # D: from o and what its rounding left off, itself rounded
+        e_ds = p * (2 * D * F32 * (dod.abs() @ vd.abs().transpose(-1, -2))
+                    + (dod.abs() * (rough + u * u * o.abs() + sub)).sum(-1, keepdim=True))
+        e_ds = e_ds + (u * u + es) * ds.abs() + see * (2.0 ** -32 * ds.abs().amax() + 2.0 ** -126)
+        tols += [u * want[1].abs() + (e_ds @ kd.abs() * scale).reshape(B, H, Tq, D) + tiny,
+                 u * want[2].abs() + (e_ds.transpose(-1, -2) @ qd.abs()).sum(2) * scale + tiny,
+                 u * want[3].abs() + dv.sum(2) + tiny]
+    return list(zip(want, tols))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("B,H,KV,T,D,window,sinks", [
+    (2, 3, 3, 1, 64, 4, 1), (2, 3, 3, 33, 64, 16, 40), (2, 4, 2, 300, 64, 100, 4), (1, 4, 1, 257, 128, None, 0),
+    (1, 4, 2, 1100, 64, 100, 4), (1, 2, 1, 1300, 128, 200, 70)])
+def test_window_attention_rounds_once(B, H, KV, T, D, window, sinks, dtype):
+    q, k, v, do = _attention_case(B, H, KV, T, T, D, dtype)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = heads.window_attention(*leaves, window, sinks)
+    got = (o,) + torch.autograd.grad(o, leaves, do)
+    for g, (w, tol), name in zip(got, _once_rounded(q, k, v, do, window, sinks), ("o", "dq", "dk", "dv")):
+        _within(g, w, tol, name)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("B,H,KV,Tq,Tk,D,window,sinks", [
+    (3, 4, 4, 1, 500, 64, None, 0), (2, 8, 2, 1, 3000, 128, None, 0), (3, 6, 3, 2, 900, 64, 128, 4),
+    (1, 16, 1, 1, 5000, 128, 2000, 33), (2, 2, 2, 40, 700, 64, 300, 2)])
+def test_window_attention_over_a_cache_rounds_once(B, H, KV, Tq, Tk, D, window, sinks, dtype):
+    q, k, v, _ = _attention_case(B, H, KV, Tq, Tk, D, dtype)
+    with torch.no_grad():
+        got = heads.window_attention(q, k, v, window, sinks)
+    (want, tol), = _once_rounded(q, k, v, None, window, sinks)
+    _within(got, want, tol, "o")
