@@ -10,9 +10,10 @@
 // One workgroup per row.  The row is read once, into registers (distill_row_kernel with NCH 16-byte
 // chunks a thread): its maximum, then both sums of exponentials, then the gradient come from there,
 // so the traffic is one read and one write of the logits, which bounds it (32768 rows of 32000 bf16
-// logits, K = 64: 850 us a pass, 4.9 TB/s, as fast as a copy of 4 GiB; before the row's floats were
-// kept from being held unpacked, at half the occupancy, 951).  Two exponentials a value in each of
-// the two passes hide behind it: at temperature 1, where one would do, the time is the same.  The K + 1 corrected places of
+// logits, K = 64: 843 - 851 us a pass, 837 of it this kernel, 5 TB/s, as fast as a copy of 4 GiB; before the
+// row's floats were kept from being held unpacked, at half the occupancy, 951).  Two exponentials a value in
+// each of the two passes just hide behind it (the vector pipe is busy for 92 % of the time): at temperature 1,
+// where one would do, the time is the same.  The K + 1 corrected places of
 // the gradient are written again after the dense pass with their whole f32 value, so each value
 // is rounded once; equal indices are added up by every entry that has them.  Sums of losses are
 // taken row by row in a fixed order (no atomics).
@@ -292,7 +293,10 @@ void launch(const DistillArgs& a, int rows, hipStream_t st) {
 
 // Threads of a row and the chunks that each holds.  Small groups: several rows of a CU then load,
 // add up and write at different times (32000 bf16 logits: 16 chunks of 256 threads 874 us, 8 of 512
-// 896, 4 of 1024 1929; 49999 f32 logits: 25 of 512 80 us, 16 of 1024 103).
+// 896, 4 of 1024 1929; 49999 f32 logits: 25 of 512 80 us, 16 of 1024 103).  At the steps' edges, 2^28 f32
+// logits: 16 of 512 (32768 columns) 441 us, 25 of 512 (33000 to 51200) 433 - 470, 16 of 1024 (51210 to
+// 65536) 526 - 584, no chunks kept (65540 to 128256) 619 - 649: that one reads three times and writes once, at
+// 6.9 TB/s (the later reads mostly from caches); bf16 338 us at 131072 columns, 388 - 410 past them.
 template <class E>
 void choose(const DistillArgs& a, int rows, hipStream_t st) {
   const int chunks = (a.V + Row<E>::N - 1) / Row<E>::N;

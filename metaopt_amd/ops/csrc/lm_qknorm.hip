@@ -10,8 +10,8 @@
 // D / 8 lanes, 16 bytes each; the mean is a butterfly over those lanes, the pairs of an
 // interleaved rotation lie within a lane and those of a rotate-half one in lane ^ (D / 16).
 // Everything is bound by memory: each value is read once and written once.  32768 rows of 36 heads
-// of 64: forward 52 us (5.8 TB/s), backward 78 us and 4 for the weights (5.2 TB/s); 12003 rows of 28
-// heads of 128: 35 (4.9 TB/s) and 57 + 5 us.
+// of 64: forward 51 us (6.0 TB/s), backward 81 us and 4 for the weights (5.0 TB/s); 12003 rows of 28
+// heads of 128: 34 (5.1 TB/s) and 57 + 6 us.
 #include "elt.h"
 
 using namespace mopt;

@@ -100,8 +100,9 @@ struct Place {
 // and what that rounding left off.  One piece alone made o, dq, dk and dv up to 1.45 times as far from 64
 // bits as outputs that are only rounded in the end; with two they are as near as these.  The price is a
 // product more for each of P V, dS K, P^T dO and dS^T Q: forward 51 -> 64 us (4 x 12 heads of 64, 4096 tokens,
-// window 512), 8192 tokens of 16 / 4 heads of 128, window 1024: 105 -> 131, dQ 144 -> 172, dK / dV 189 -> 246;
-// a single token over a cache 15.0 -> 15.1, memory bounds that.
+// window 512), 8192 tokens of 16 / 4 heads of 128, window 1024: 89 -> 112, dQ 123 -> 146, dK / dV 158 -> 206;
+// 125M step (64 x 12 heads of 64, 512 tokens, window 128): 57 -> 60, 78 -> 82, 81 -> 92; a single token over
+// a cache 14.8 -> 15.0, memory bounds that.  (Medians of 300 passes by the profiler, as all times here.)
 struct Two {
   u32x4 hi, lo;
 };
@@ -313,7 +314,7 @@ __device__ __forceinline__ void hide(f32x16& x, float with, int i, int k0, int l
 // each row of a product (dQ: a query, dK: a key) carries a power of two of its own: dS comes multiplied by
 // it, and where a row's largest passes 2^15 the factor, this group and the sums so far are brought down to
 // put it at 2^7 ... 2^8.  A pair is then off by 2^-11 of itself or 2^-32 of its row's largest.  It starts at
-// 2^60: products of fp16 rows (below 2^39) stay inside 32 bits with it.
+// 2^60: products of fp16 rows (below 2^39) stay inside 32 bits with it.  It costs dQ 3 - 6 %, dK / dV 8 %.
 constexpr float kFirstLift = (float)(1ull << 60);
 
 // the factor that `x`, its row's sums and its lift take now (1, mostly)
@@ -330,11 +331,10 @@ __device__ __forceinline__ float settle(f32x16& x) {
   return f;
 }
 
-// Forward: one pass over the keys with a running reference and sum.  Heads of 64 (4 sequences of 12
-// heads, 4096 tokens, window 512: 51 us, 475 TFLOP/s) are bound by the vector work on the scores, on a
-// SIMD about 670 clocks a group of 32 x 32 pairs, and 256 of products that hardly overlap with it: 940.
-// Heads of 128 (8192 tokens of 16 / 4 heads, window 1024: 101 us, 640 TFLOP/s) by both: 660 + 512
-// clocks of 1320, with 2 waves a SIMD or 3 (tiles of 32 keys).
+// Forward: one pass over the keys with a running reference and sum.  Bound by the vector work on the scores
+// and the products, which hardly overlap: heads of 64 (4 sequences of 12 heads, 4096 tokens, window 512: 64
+// us, passes back to back 57) keep the vector pipe busy for 47 % of the time and the matrix pipe for 27 %,
+// heads of 128 (8192 tokens of 16 / 4 heads, window 1024: 112 us) both for 37 %.
 template <class E, int D>
 __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a, uint16_t* o, uint16_t* rest,
                                                                        float* lse) {
@@ -447,9 +447,9 @@ __global__ __launch_bounds__(256, kFwdWaves<D>) void window_fwd_kernel(WinArgs a
 // dQ, and D of its rows for the dK / dV kernel.  D is formed from o and what o's rounding left off
 // (`rest`, written by the forward): with o alone its error adds to that of the rounded dS, and where
 // few keys are seen it is the larger one (a window of 4: 1.8 times the error of a once rounded dq
-// instead of 1.5).  125M step (64 x 12 heads, 512 tokens, window 128): 84 us, of which reading and
-// writing 350 MB is 65; heads of 128, 8192 tokens, window 1024: 137 us (705 TFLOP/s),
-// products and vector work as above.
+// instead of 1.5, with dS in one piece).  125M step (64 x 12 heads, 512 tokens, window 128): 82 us, of which
+// reading and writing 356 MB is 66; heads of 128, 8192 tokens, window 1024: 146 us, the matrix pipe busy for
+// 38 % of it, the vector pipe for 31 %.
 template <class E, int D>
 __global__ __launch_bounds__(256, kDqWaves<D>) void window_dq_kernel(WinArgs a, const uint16_t* o,
                                                                      const uint16_t* rest, const uint16_t* dout,
@@ -587,11 +587,10 @@ __device__ __forceinline__ u32x4 pieces(float v, int lane) {
 // turns at the groups of 32 queries.
 // What is not a key's whole sum is left in 32 bits: the near sums of all rows (parts > 1) or of rows
 // j < S, [part][b, hk][rows][2][D], and the far ones behind them, [span][wave][b, hk][S][2][D];
-// window_sum_kernel adds them.  125M step (64 x 12 heads, 512 tokens, window 128, 4 sinks): 94 us, bound
-// by the vector work on the scores (exp2, dS, packing) and the products, which hardly overlap; 8192
-// tokens of 16 / 4 heads, window 1024: heads of 64 108 us, of 128 189 us (six such sequences 880: 147
-// each, 880 TFLOP/s).  (Two waves for each key, 8 a workgroup, were slower
-// everywhere: 125M step 272 us.)
+// window_sum_kernel adds them.  125M step (64 x 12 heads, 512 tokens, window 128, 4 sinks): 92 us, of which
+// reading and writing 397 MB is 74; 8192 tokens of 16 / 4 heads, window 1024: heads of 64 124 us, of 128 206
+// us, the matrix pipe busy for 42 % of it, the vector pipe for 29 % (six such sequences 1171: 195 each).
+// (Two waves for each key, 8 a workgroup, were nearly 3 times slower.)
 template <class E, int D>
 struct Dkv {
   // heads of 128: 64 registers of key and value fragments beside 128 of sums leave too few for the
@@ -702,8 +701,8 @@ struct Dkv {
   __device__ __forceinline__ void step(int slot, int sub, bool all, int d0, uint32_t mine) {
     const uint32_t Qs = lds_at(lds.ring[slot][0]) + sub * 64 * D, Os = lds_at(lds.ring[slot][1]) + sub * 64 * D;
     // Both products start at what their rows' sums take off: a value of each row in three pieces, times
-    // ones.  (From LDS to the registers that need them the 2 x 16 values would be 8 reads of 1 KB: heads
-    // of 64, 8192 tokens of 4 key heads, window 1024: 123 us so, 110 this way.)
+    // ones.  (From LDS to the registers that need them the 2 x 16 values would be 8 reads of 1 KB, 12 % of
+    // the time of heads of 64.)
     const int own = 32 * sub + swap23(lane & 31);
     const u32x4 ones = {0x3F803F80, 0x3F803F80, 0x3F803F80, 0x3F803F80};
     f32x16 x = Bf16::mfma32(pieces(-lds.stat[slot][0][own] * rc, lane), ones, zero16());
@@ -865,12 +864,12 @@ __global__ __launch_bounds__(256) void window_sum_kernel(const float* part, int 
 // that go through the keys 32 at a time on their own -- keys from memory into registers as operands,
 // values into LDS for the transposing read, both a chunk ahead -- and join their maxima, sums and
 // products in the end.  With `splits` > 1 the keys of a head are shared among that many workgroups,
-// which leave theirs in `part`, and window_join_kernel joins them.  32768 keys of 8 heads of 128: 25.5 us
+// which leave theirs in `part`, and window_join_kernel joins them.  32768 keys of 8 heads of 128: 25.2 us
 // (5.3 TB/s) and 4 for joining.
 // Products are 16x16x32: lane l holds A[l & 15][8 (l >> 4) ..], B[8 (l >> 4) ..][l & 15] and
 // C[4 (l >> 4) + r][l & 15]; the keys of the two score tiles of a chunk are fed so that a lane's
 // 4 + 4 scores are those of keys 8 (l >> 4) ... + 7, the B operand of the product with V.
-constexpr int NW = 8;          // (64 sequences of 4 key heads of 64, 1028 keys: 13.8 us, with 16 waves 15.3)
+constexpr int NW = 8;          // (64 sequences of 4 key heads of 64, 1028 keys: 15.0 us, with 16 waves 10 % more)
 
 __device__ __forceinline__ float over_groups(float v, bool mx) {      // lanes l, l ^ 16, l ^ 32, l ^ 48
   const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -377,9 +377,9 @@ def window_attention_ref(q, k, v, window=None, sinks=0, scale=None, start=None, 
 
 def _span(sinks: int, heads: int, Tq: int) -> int:
     """Queries of one item of the dK / dV kernel that adds up sinks' pairs out of the window
-    (csrc/lm_window.hip): 512 where there are so many of these that they fill the CUs (125M step: 91
-    us, with 128 117), else 128, as the others wait for the last of them (8192 tokens, 4 key heads of
-    128: 189 us, with 512 225); and so many that the 4 partial sums of the sinks' rows that each
+    (csrc/lm_window.hip): 512 where there are so many of these that they fill the CUs (125M step: 95
+    us, with 128 107), else 128, as the others wait for the last of them (8192 tokens, 4 key heads of
+    128: 206 us, with 512 264); and so many that the 4 partial sums of the sinks' rows that each
     leaves are no more than there are queries."""
     near = 512 if heads * -(-Tq // 512) >= 256 else 128
     return max(near, -(-4 * sinks // 64) * 64)
@@ -391,7 +391,7 @@ def _geometry(q, k, v):
 
 def _splits(heads: int, tokens: int) -> int:
     """Workgroups that share the ``tokens`` keys of each of ``heads`` key heads: at most one a CU
-    over all heads (32768 keys of 8 heads: 26 us, with two a CU 30), and each with 1024 keys at
+    over all heads (32768 keys of 8 heads: 25 us, with two a CU 29), and each with 1024 keys at
     least: joining them costs a launch, 3.4 us, as much as about 1000 keys do."""
     return max(1, min(256 // heads, tokens // 1024))
 
@@ -422,7 +422,7 @@ def _window_fwd(q, k, v, window, sinks, scale, start, start0, lengths, train):
 def _parts(blocks: int, steps: int) -> int:
     """Workgroups that share the queries of each of ``blocks`` key blocks in the dK / dV kernel,
     where there are fewer blocks than two a CU (8192 tokens of 4 key heads, window 1024: heads of 64
-    123 + 9 us against 167, of 128 189 + 14 against 226), each with 8 of the block's ``steps``
+    124 + 8 us against 171 + 5, of 128 206 + 14 against 240 + 6), each with 8 of the block's ``steps``
     groups of 32 queries at least.  Their sums are added up by another launch."""
     return max(1, min(512 // max(1, blocks), steps // 8))
 
