@@ -52,7 +52,6 @@ class TaskSpec:
         if self.needs_fidelity and not fids:
             raise ValueError("this task needs a /steps fidelity (its trials' budgets)")
 
-
     def parse_options(self, text) -> dict:
         """The arguments of ``build`` in the JSON object ``text`` (None: none)."""
         if not text:
